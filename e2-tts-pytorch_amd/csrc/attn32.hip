@@ -257,9 +257,9 @@ __global__ __launch_bounds__(256, 4) void attn_fwd32_kernel(AttnArgs p) {
                 fwd_block<2, DROP, SHARE, true, PROBE>(s, kb, cc, lsum2, hk, p.thresh, kmb, pf, mk);
             }
             if (DROP && SHARE) {
-                // the compare masks of the block (SGPR pairs) leave through the scalar data cache: no vector instruction
+                // the compare masks of the block (SGPR pairs) leave as one 128-byte vector store
                 unsigned long long* dw = p.dropbits + (((long)bh * nt + kt) * nqb + qb) * 32 + 16 * kb;
-                sstore_masks16(dw, mk);
+                store_masks16(dw, mk, lane);
             }
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2) {
@@ -272,7 +272,6 @@ __global__ __launch_bounds__(256, 4) void attn_fwd32_kernel(AttnArgs p) {
             }
         }
     }
-    if (DROP && SHARE) sstore_flush();     // (every wave: write the scalar data cache back before the kernel ends)
     float lsum = (lsum2[0][0] + lsum2[0][1]) + (lsum2[1][0] + lsum2[1][1]);
     if (!live) return;
     lsum += lane32_other(lsum);                 // a row's keys are split over lanes l and l + 32

@@ -197,39 +197,29 @@ template <int N> __device__ __forceinline__ void wave_sum_rows(float (&v)[N]) {
 // value index held by register i of the lanes of row r after wave_sum_rows<N>
 template <int N> __device__ __forceinline__ constexpr int wave_sum_rows_index(int i, int r) { return i + (N / 4) * (r & 1) + (N / 2) * (r >> 1); }
 
-// 16 wave masks (SGPR pairs, e.g. fresh from v_cmp) -> 128 consecutive bytes at a wave-uniform address, through the scalar data cache
-// (s_store_dwordx2: no vector instruction, no VGPR).  The statement waits for its own stores (lgkmcnt) before the SGPRs may be reused;
-// the leading s_nop covers a VALU write of an SGPR read by the scalar memory instruction.  The cache is written back by
-// sstore_flush(), which every wave that stored must execute before it ends.
-template <bool WAIT = true>
-__device__ __forceinline__ void sstore_masks16(unsigned long long* dst, const unsigned long long (&m)[16]) {
-    typedef __attribute__((address_space(1))) unsigned long long* gp_t;
-#define E2K_SST16_ \
-        "s_nop 4\n" \
-        "s_store_dwordx2 %1, %0, 0x0\n s_store_dwordx2 %2, %0, 0x8\n s_store_dwordx2 %3, %0, 0x10\n s_store_dwordx2 %4, %0, 0x18\n" \
-        "s_store_dwordx2 %5, %0, 0x20\n s_store_dwordx2 %6, %0, 0x28\n s_store_dwordx2 %7, %0, 0x30\n s_store_dwordx2 %8, %0, 0x38\n" \
-        "s_store_dwordx2 %9, %0, 0x40\n s_store_dwordx2 %10, %0, 0x48\n s_store_dwordx2 %11, %0, 0x50\n s_store_dwordx2 %12, %0, 0x58\n" \
-        "s_store_dwordx2 %13, %0, 0x60\n s_store_dwordx2 %14, %0, 0x68\n s_store_dwordx2 %15, %0, 0x70\n s_store_dwordx2 %16, %0, 0x78\n"
-#define E2K_SST16_OPS_ \
-        :: "s"((gp_t)dst), "s"(m[0]), "s"(m[1]), "s"(m[2]), "s"(m[3]), "s"(m[4]), "s"(m[5]), "s"(m[6]), "s"(m[7]), \
-           "s"(m[8]), "s"(m[9]), "s"(m[10]), "s"(m[11]), "s"(m[12]), "s"(m[13]), "s"(m[14]), "s"(m[15]) : "memory"
-    if (WAIT) asm volatile(E2K_SST16_ "s_waitcnt lgkmcnt(0)" E2K_SST16_OPS_);
-    else asm volatile(E2K_SST16_ "s_nop 0" E2K_SST16_OPS_);          // (probe: are the data SGPRs read at issue?)
-#undef E2K_SST16_
-#undef E2K_SST16_OPS_
-}
-// eight masks (64 bytes)
-__device__ __forceinline__ void sstore_masks8(unsigned long long* dst, unsigned long long m0, unsigned long long m1, unsigned long long m2, unsigned long long m3,
-                                              unsigned long long m4, unsigned long long m5, unsigned long long m6, unsigned long long m7) {
-    typedef __attribute__((address_space(1))) unsigned long long* gp_t;
+// 16 wave-uniform dwords -> one register, dword i in lane i (v_writelane; lanes 16 .. 63 keep `old`).  The leading s_nop covers SGPRs that a
+// v_cmp has just written (the compiler does not look into the statement).
+__device__ __forceinline__ unsigned lanes_from16(unsigned old, const unsigned (&m)[16]) {
     asm volatile(
         "s_nop 4\n"
-        "s_store_dwordx2 %1, %0, 0x0\n s_store_dwordx2 %2, %0, 0x8\n s_store_dwordx2 %3, %0, 0x10\n s_store_dwordx2 %4, %0, 0x18\n"
-        "s_store_dwordx2 %5, %0, 0x20\n s_store_dwordx2 %6, %0, 0x28\n s_store_dwordx2 %7, %0, 0x30\n s_store_dwordx2 %8, %0, 0x38\n"
-        "s_waitcnt lgkmcnt(0)"
-        :: "s"((gp_t)dst), "s"(m0), "s"(m1), "s"(m2), "s"(m3), "s"(m4), "s"(m5), "s"(m6), "s"(m7) : "memory");
+        "v_writelane_b32 %0, %1, 0\n v_writelane_b32 %0, %2, 1\n v_writelane_b32 %0, %3, 2\n v_writelane_b32 %0, %4, 3\n"
+        "v_writelane_b32 %0, %5, 4\n v_writelane_b32 %0, %6, 5\n v_writelane_b32 %0, %7, 6\n v_writelane_b32 %0, %8, 7\n"
+        "v_writelane_b32 %0, %9, 8\n v_writelane_b32 %0, %10, 9\n v_writelane_b32 %0, %11, 10\n v_writelane_b32 %0, %12, 11\n"
+        "v_writelane_b32 %0, %13, 12\n v_writelane_b32 %0, %14, 13\n v_writelane_b32 %0, %15, 14\n v_writelane_b32 %0, %16, 15\n"
+        : "+v"(old)
+        : "s"(m[0]), "s"(m[1]), "s"(m[2]), "s"(m[3]), "s"(m[4]), "s"(m[5]), "s"(m[6]), "s"(m[7]), "s"(m[8]), "s"(m[9]), "s"(m[10]), "s"(m[11]),
+          "s"(m[12]), "s"(m[13]), "s"(m[14]), "s"(m[15]));
+    return old;
 }
-__device__ __forceinline__ void sstore_flush() { asm volatile("s_dcache_wb\n s_waitcnt lgkmcnt(0)" ::: "memory"); }
+// 16 wave masks (SGPR pairs, e.g. fresh from v_cmp) -> 128 consecutive bytes at a wave-uniform address: lane i collects mask i, lanes
+// 0 .. 15 store eight bytes each
+__device__ __forceinline__ void store_masks16(unsigned long long* dst, const unsigned long long (&m)[16], int lane) {
+    unsigned lo[16], hi[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) { lo[i] = (unsigned)m[i]; hi[i] = (unsigned)(m[i] >> 32); }
+    const unsigned a = lanes_from16(0u, lo), b = lanes_from16(0u, hi);
+    if (lane < 16) dst[lane] = ((unsigned long long)b << 32) | a;
+}
 
 // counted wait on outstanding vector-memory ops (LDS-DMA included) and a raw workgroup barrier that does NOT drain
 // them: lets global_load_lds prefetches stay in flight across barriers (cdna_hip_programming.md T3+T4)

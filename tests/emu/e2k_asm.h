@@ -127,15 +127,7 @@ template <int N> inline void wave_sum_rows(float (&v)[N]) {      // same swap / 
 }
 template <int N> inline constexpr int wave_sum_rows_index(int i, int r) { return i + (N / 4) * (r & 1) + (N / 2) * (r >> 1); }
 
-template <bool WAIT = true>
-inline void sstore_masks16(unsigned long long* dst, const unsigned long long (&m)[16]) {      // (every lane writes the same 128 bytes)
-    for (int i = 0; i < 16; ++i) dst[i] = m[i];
-}
-inline void sstore_masks8(unsigned long long* dst, unsigned long long m0, unsigned long long m1, unsigned long long m2, unsigned long long m3,
-                          unsigned long long m4, unsigned long long m5, unsigned long long m6, unsigned long long m7) {
-    dst[0] = m0; dst[1] = m1; dst[2] = m2; dst[3] = m3; dst[4] = m4; dst[5] = m5; dst[6] = m6; dst[7] = m7;
-}
-inline void sstore_flush() {}
+inline void store_masks16(unsigned long long* dst, const unsigned long long (&m)[16], int lane) { if (lane < 16) dst[lane] = m[lane]; }
 inline void wait_lgkm0() {}
 template <int N> inline void wait_vmcnt() { emu::land_pending(N); }
 inline void barrier_keep_vm() { emu::block_rendezvous(); }

@@ -1,5 +1,5 @@
 """What bounds attn_fwd32_kernel?  Bottleneck probes (E2K_ATTN32_PROBE bits: results are wrong on purpose) at the bench shape, dropout 0.1,
-masks published by scalar stores.  1 no exp2, 2 no counter hash, 4 no score MFMAs, 8 no LDS fragment reads, 16 no output MFMAs,
+keep masks published.  1 no exp2, 2 no counter hash, 4 no score MFMAs, 8 no LDS fragment reads, 16 no output MFMAs,
 32 no LDS-DMA after the first two tiles, 64 no barriers.  -> gpurun_out/r05_attn32_ablate.json"""
 import json
 import os
