@@ -20,6 +20,14 @@ OBJ = HERE / 'build'
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-ffp-contract=fast',
          '-I', str(ROOT / 'include'), '-I', str(CSRC)]
+# Sources added since hipcc's packed-fp32 instructions were found to misbehave next to LDS-DMA traffic (tests/test_abi.py) are compiled without
+# them; the older ones keep the code they were measured and fenced with.
+NO_PACKED_FP32 = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
+NO_PACKED = {'layernorm.hip', 'packed_attn.hip'}
+
+
+def _flags(src):
+    return FLAGS + (NO_PACKED_FP32 if src.name in NO_PACKED else [])
 
 
 def _digest(paths):
@@ -27,7 +35,7 @@ def _digest(paths):
     for p in sorted(paths):
         h.update(p.name.encode())
         h.update(p.read_bytes())
-    h.update(' '.join(FLAGS).encode())
+    h.update(' '.join(FLAGS + NO_PACKED_FP32 + sorted(NO_PACKED)).encode())
     return h.hexdigest()
 
 
@@ -44,10 +52,10 @@ def build(force: bool = False, verbose: bool = True) -> Path:
     def compile_one(src: Path):
         obj = OBJ / (src.stem + '.o')
         ostamp = OBJ / (src.stem + '.stamp')
-        d = hashlib.sha256(src.read_bytes() + hdr_dig.encode()).hexdigest()
+        d = hashlib.sha256(src.read_bytes() + hdr_dig.encode() + ' '.join(_flags(src)).encode()).hexdigest()
         if not force and obj.exists() and ostamp.exists() and ostamp.read_text() == d:
             return obj
-        cmd = [HIPCC, *FLAGS, '-c', str(src), '-o', str(obj)]
+        cmd = [HIPCC, *_flags(src), '-c', str(src), '-o', str(obj)]
         if verbose:
             print('[e2k build]', ' '.join(cmd), flush=True)
         subprocess.run(cmd, check=True)

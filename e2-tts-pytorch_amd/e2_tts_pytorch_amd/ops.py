@@ -624,6 +624,84 @@ def rmsnorm_bwd(dy, x, rn, gamma, gamma_off, rows_per_batch, dgamma):
     return dx
 
 
+def _ln_cols(t, M, D, rows_per_batch, what):
+    """checks a (D,) or (batch elements, D) fp32 column vector of a layer norm -> 2-D view"""
+    if t.dim() == 1:
+        t = t[None]
+    need = -(-M // rows_per_batch)
+    if t.dtype != f32 or t.dim() != 2 or t.shape[1] != D or t.shape[0] < need or (D > 1 and t.stride(1) != 1):
+        raise E2KError(f'layer norm: {what} must be fp32 ({need} or more, {D}) with contiguous rows, got {t.dtype} {tuple(t.shape)}')
+    return t
+
+
+def _ln_rows(x, what):
+    if x.dim() != 2 or x.dtype not in (bf16, f32) or (x.shape[1] > 1 and x.stride(1) != 1) or not 1 <= x.shape[1] <= 8192:
+        raise E2KError(f'layer norm: {what} must be (rows, 1 .. 8192 columns) bf16 or fp32 with contiguous rows, got {x.dtype} {tuple(x.shape)}')
+    if x.shape[0] > 1 and x.stride(0) < x.shape[1]:
+        raise E2KError(f'layer norm: rows of {what} overlap')
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def layernorm_fwd(x, gamma, beta, gamma_off=0., rows_per_batch=0, eps=1e-5):
+    """x (M,D) bf16 or fp32, rows may be strided; gamma / beta fp32 (D,), (nb,D) or None; row m takes gamma / beta row m // rows_per_batch (0: one
+    row for all).  -> (y, mean (M,), rstd (M,)): y contiguous with x's type, mean / rstd fp32 for layernorm_bwd"""
+    _chk(x, gamma, beta)
+    ldx = _ln_rows(x, 'x')
+    M, D = x.shape
+    rpb = int(rows_per_batch) or max(M, 1)
+    if rpb < 0 or not eps >= 0:
+        raise E2KError('layer norm: rows_per_batch and eps must not be negative')
+    gamma = None if gamma is None else _ln_cols(gamma, M, D, rpb, 'gamma')
+    beta = None if beta is None else _ln_cols(beta, M, D, rpb, 'beta')
+    if gamma is not None and beta is not None and gamma.shape[0] > 1 and gamma.stride(0) != beta.stride(0):
+        beta = beta.contiguous()
+        gamma = gamma.contiguous()
+    ldg = next((t.stride(0) for t in (gamma, beta) if t is not None), D)
+    y = torch.empty((M, D), dtype=x.dtype, device=x.device)
+    mean, rstd = torch.empty((2, M), dtype=f32, device=x.device).unbind(0)
+    _lib.get().e2k_layernorm_fwd(_p(x), ldx, int(x.dtype == f32), _p(gamma), _p(beta), ldg, float(gamma_off), rpb, float(eps), _p(y), _p(mean), _p(rstd),
+                                 M, D, _stream(x))
+    return y, mean, rstd
+
+
+def layernorm_bwd(dy, x, mean, rstd, gamma, gamma_off=0., rows_per_batch=0, dgamma=None, dbeta=None, need_weights=True):
+    """-> (dx, dgamma, dbeta): dx contiguous with x's type; dgamma / dbeta fp32 (nb,D) are ADDED TO where given, fresh where not (None for both with
+    need_weights=False)"""
+    _chk(dy, x, mean, rstd, gamma, dgamma, dbeta)
+    ldx = _ln_rows(x, 'x')
+    M, D = x.shape
+    rpb = int(rows_per_batch) or max(M, 1)
+    nb = -(-M // rpb)
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise E2KError(f'layer norm: dy must match x, got {dy.dtype} {tuple(dy.shape)} for {x.dtype} {tuple(x.shape)}')
+    dy = dy.contiguous()
+    for t in (mean, rstd):
+        if t.dtype != f32 or t.shape != (M,) or not t.is_contiguous():
+            raise E2KError('layer norm: mean and rstd are the forward\'s')
+    gamma = None if gamma is None else _ln_cols(gamma, M, D, rpb, 'gamma')
+    dx = torch.empty((M, D), dtype=x.dtype, device=x.device)
+    ws, ldd, acc = None, D, 0
+    if need_weights:
+        if (dgamma is None) != (dbeta is None):
+            raise E2KError('layer norm: give both dgamma and dbeta or neither')
+        if dgamma is None:
+            dgamma, dbeta = (torch.zeros if M == 0 else torch.empty)((2, nb, D), dtype=f32, device=x.device).unbind(0)
+        else:
+            acc = 1
+            _ln_cols(dgamma, M, D, rpb, 'dgamma'), _ln_cols(dbeta, M, D, rpb, 'dbeta')
+            if dgamma.shape != dbeta.shape or dgamma.stride() != dbeta.stride():
+                raise E2KError('layer norm: dgamma and dbeta must have the same shape and strides')
+            if dgamma.dim() == 2 and dgamma.shape[0] > 1 and dgamma.stride(0) < D:
+                raise E2KError('layer norm: rows of dgamma overlap')
+        ldd = dgamma.stride(0) if dgamma.dim() == 2 else D
+        ws = torch.empty(_lib.get().e2k_query_layernorm_bwd_ws_floats(M, D, rpb), dtype=f32, device=x.device)
+    elif dgamma is not None or dbeta is not None:
+        raise E2KError('layer norm: dgamma / dbeta given with need_weights=False')
+    _lib.get().e2k_layernorm_bwd(_p(dy), _p(x), ldx, int(x.dtype == f32), _p(mean), _p(rstd), _p(gamma), gamma.stride(0) if gamma is not None else D,
+                                 float(gamma_off), rpb, _p(dx), _p(dgamma), _p(dbeta), ldd, acc, _p(ws), M, D, _stream(x))
+    return dx, dgamma, dbeta
+
+
 def gate_bwd(dy, y, g, gsum, rows_per_batch):
     _chk(dy, y, g, gsum)
     M, D = y.shape

@@ -175,6 +175,20 @@ int e2k_rmsnorm_bwd(const void* dy, const void* x, const float* rn, const float*
                     float gamma_off, int rows_per_batch, void* dx, float* dgamma, int M, int D,
                     void* stream);
 
+/* ---- LayerNorm (beside RMSNorm: the norm of blocks next to the backbone, e.g. the vocoder's, and of adaptive "scale and shift" blocks) ----
+ * y = (x - mean) * rstd * (gamma[m / rows_per_batch] + gamma_off) + beta[m / rows_per_batch],  rstd = 1 / sqrt(var + eps), var over the D columns
+ * x rows ldx elements apart, bf16 (dtype 0) or fp32 (dtype 1); y contiguous, the type of x.  gamma / beta fp32, one row of D per batch element
+ * (ldg floats apart) or one for all (rows_per_batch >= M); NULL = 1 / 0 (gamma_off then unused).  mean / rstd (M) fp32 for the backward, both or
+ * neither.  1 <= D <= 8192, any alignment (rows that are multiples of 16 bytes take wide accesses). */
+int e2k_layernorm_fwd(const void* x, int64_t ldx, int dtype, const float* gamma, const float* beta, int64_t ldg, float gamma_off,
+                      int rows_per_batch, float eps, void* y, float* mean, float* rstd, int M, int D, void* stream);
+/* dx (contiguous, type of x) and, where asked for (either may be NULL), dgamma / dbeta (fp32, rows ldd apart; added to with accumulate = 1).
+ * ws: e2k_query_layernorm_bwd_ws_floats floats (NULL when neither is asked for).  Sums in a fixed order: the same bits every time. */
+int64_t e2k_query_layernorm_bwd_ws_floats(int M, int D, int rows_per_batch);
+int e2k_layernorm_bwd(const void* dy, const void* x, int64_t ldx, int dtype, const float* mean, const float* rstd, const float* gamma,
+                      int64_t ldg, float gamma_off, int rows_per_batch, void* dx, float* dgamma, float* dbeta, int64_t ldd, int accumulate,
+                      float* ws, int M, int D, void* stream);
+
 /* AdaLN-Zero gate backward (AdaLNZero, e2_tts.py:346-351; the forward multiply is the colscale epilogue of
  * e2k_gemm_nt_bf16):  dao = dy * g[b];  gsum[b][d] += sum_rows dy * y   (y = gated output, g = sigmoid gate) */
 int e2k_gate_bwd(const void* dy, const void* y, const float* g, void* dao, float* gsum, int64_t ldg,
