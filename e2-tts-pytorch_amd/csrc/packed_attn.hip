@@ -1,0 +1,950 @@
+// Attention over packed documents, forward and backward (dim_head 64).
+//
+// Queries and keys of several documents lie one behind the other on one token axis; document d's queries are rows cu_q[d] .. and its keys
+// rows cu_k[d] .. (optionally only the first len_q[d] / len_k[d] of that slot).  Query i of a document with nq queries and nk keys stands at
+// position i + nk - nq (the last query on the last key) and sees the keys j < lim(i):
+//     full: nk       causal: min(nk, max(position + 1, prefix))
+// Per visible pair    z = scale q.k;   c = cap tanh(z / cap)  (cap > 0);   t = c - slope_h |j - position|   or   t = c + table[bucket(j - position), h]
+//                     p = softmax(t);  o = p v;   a row that sees nothing has o = 0
+// Backward            dS = p (dO.v - dO.o);  dtable[b, h] = sum of dS over the pairs of bucket b;  dz = dS (1 - tanh^2) scale
+//                     dq = dz k;  dk = dz^T q;  dv = p^T dO      (grouped heads: dk, dv summed over the query heads of a key head)
+//
+// Layout: as in attn32.hip a wave owns 32 rows (lane = one query in the forward and dQ kernels, one key in the dK / dV kernel) on 32x32x16
+// MFMAs, the scores computed swapped so that a lane's accumulators are the B operand of the next product.  Here the second operands come out
+// of the row-major tiles by transposing LDS reads (no V^T copy is needed: packed rows are read as they lie, any token and head stride).
+//
+// What a wave does per 32-key block beyond the products is a few vector operations per score, and the bias is arranged to cost next to none of
+// them: where a block lies wholly on one side of its queries the linear bias splits into a per-lane constant (folded into the running maximum)
+// and sixteen wave-uniform addends (the addend of the multiply-add that scales the score anyway); where a block lies beyond the table's reach
+// the learned bias is one constant.  Only blocks that cross the diagonal (or lie within reach) take |distance| (an LDS lookup) per score.
+//
+// Softmax: running maximum with a lazy rescale -- the accumulators are rescaled only when a block's maximum exceeds the reference point by 2^8
+// (fp32 sums and bf16 probabilities lose nothing by a common factor), which in practice happens in the first block or two of a row.
+// The table's gradient is a sum of the small differences p (dO.v - dO.o) over every pair at a distance, returned in fp32: an o that is good to
+// bf16 only (probabilities rounded before the second product, output rounded after it) would show in its third digit.  A training forward with
+// a table therefore carries the probabilities as two bf16 terms through the second product and keeps what rounding cut off the output (o_lo):
+// dO.o is then good to 2^-16 of its terms.
+//
+// Sums are taken in a fixed order throughout: no atomics, the same bits every time.
+#include "e2k_device.h"
+#include "plan.h"
+#include <e2k_asm.h>
+#include "../../include/e2k.h"
+#include "attn_tile32.h"
+
+using namespace e2k;
+
+namespace {
+
+constexpr int DH = 64;
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+constexpr int STAGE = 16384;          // one ring stage: two [64][64] bf16 tiles
+constexpr float M_INIT = -1e30f;      // running maximum before any visible key
+constexpr float LSE_EMPTY = 1e30f;    // log-sum-exp of a row that sees nothing: exp2(t - it) is 0
+constexpr float M_SLACK = 8.f;        // (log2) how far a score may exceed the reference point before the accumulators are rescaled
+constexpr int PADL = 64;              // entries of the distance table beyond its reach on either side (a block's distances spread over 63)
+constexpr int REACH_MAX = 512;
+constexpr int GAP_PARTS = 8;          // workgroups per gap between documents
+
+struct PAArgs {
+    const bf16_t *Q, *K, *V, *dO;
+    long sq, hq, sk, hk, sv, hv, so, ho, sg, hg;       // token and head strides (elements) of Q, K, V, O, dO
+    const int *cu_q, *cu_k, *len_q, *len_k, *prefix;
+    int nd, Tq, Tk, H, Hkv, G;
+    float scale, cap;
+    int causal, fill;
+    const float *slopes, *table; const int* buckets; int nbuckets, R;
+    bf16_t *O, *Olo;                                   // O strided; Olo (Tq, H, 64)
+    float *lse2, *delta;                               // (H, Tq)
+    bf16_t *dQ, *dK, *dV;                              // (Tq, H, 64), (Tk, Hkv, 64)
+    float* dist;                                       // [workgroup of the dQ grid][2 R + 1]: sums of dS by distance
+    int nt, nwork;                                     // row tiles per (document, head) of this grid; workgroups that compute
+};
+
+__device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
+// rows of document d, kept inside [0, total) whatever the offsets say
+struct Span { int at, n; };
+__device__ __forceinline__ Span span(const int* cu, const int* len, int d, int total) {
+    Span s;
+    s.at = clampi(cu[d], 0, total);
+    const int end = clampi(cu[d + 1], s.at, total);
+    s.n = end - s.at;
+    if (len) s.n = clampi(len[d], 0, s.n);
+    return s;
+}
+struct Doc {
+    int q0, nq, k0, nk, off, prefix, causal;
+    __device__ __forceinline__ int lim(int i) const {           // keys that query i sees: 0 .. lim(i) - 1 (never falls with i)
+        if (!causal) return nk;
+        const int a = i + off + 1;
+        return clampi(a > prefix ? a : prefix, 0, nk);
+    }
+};
+__device__ __forceinline__ Doc doc_of(const PAArgs& p, int d) {
+    const Span a = span(p.cu_q, p.len_q, d, p.Tq), b = span(p.cu_k, p.len_k, d, p.Tk);
+    Doc r{uniform_i(a.at), uniform_i(a.n), uniform_i(b.at), uniform_i(b.n), 0, 0, p.causal};
+    r.off = r.nk - r.nq;
+    r.prefix = (p.causal && p.prefix) ? uniform_i(clampi(p.prefix[d], 0, r.nk)) : 0;
+    return r;
+}
+
+// Workgroups go to the 8 XCDs round-robin in launch order.  Re-numbered so that an XCD gets a contiguous run of (head, document, tile): the
+// tiles of a (document, head) stream the same K / V through one L2, and with eight or more heads every XCD has all documents (equal work).
+struct Work { int h, d, tile, lin; };
+__device__ __forceinline__ Work work_of(const PAArgs& p) {
+    const int q = p.nwork >> 3, r = p.nwork & 7;
+    int lin = (int)blockIdx.x;
+    const int xcd = lin & 7;
+    lin = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (lin >> 3);
+    Work w;
+    w.lin = lin;
+    w.tile = p.nt - 1 - lin % p.nt;          // causal: the long rows first
+    const int hd = lin / p.nt;
+    w.d = hd % p.nd;
+    w.h = hd / p.nd;
+    return w;
+}
+
+// rows that no document covers, between documents d - 1 and d (d = nd: behind the last): zeros
+__device__ __forceinline__ void fill_gap(const int* cu, const int* len, int nd, int total, bf16_t* out, long ts, long hs, int nh, int id) {
+    const int g = id / GAP_PARTS, part = id % GAP_PARTS;
+    int from = 0;
+    if (g > 0) {
+        const Span s = span(cu, len, g - 1, total);
+        from = s.at + s.n;
+    }
+    const int to = g < nd ? clampi(cu[g], 0, total) : total;
+    for (int row = from + part; row < to; row += GAP_PARTS)
+        for (int c = threadIdx.x; c < nh * 8; c += blockDim.x)
+            st<u32x4>(out + (long)row * ts + (long)(c >> 3) * hs + (c & 7) * 8, u32x4{0u, 0u, 0u, 0u});
+}
+
+// ------------------------------------------------------------------------------------------------ scores
+
+__device__ __forceinline__ constexpr int reg_off(int r) { return 16 * (r >> 3) + (r & 7); }      // row of accumulator r within its block (+ 8 hi)
+
+// tanh cap:  out tanh(s kx)  with out = cap log2(e).  |s kx| <= 0.3 (a wave vote): minimax of tanh(x) / x in x^2, four terms, relative error
+// 1e-8 (below fp32's half step); beyond: 1 - 2 / (2^(2 x log2 e) + 1)
+constexpr float CAP_POLY_MAX = 0.3f;
+struct Cap { float a0, a1, a2, a3, k2, out, lim; };
+__device__ __forceinline__ Cap cap_of(float scale, float cap) {
+    Cap c;
+    const float kx = scale / cap, k2 = kx * kx;
+    c.out = cap * LOG2E;
+    const float k1 = c.out * kx;
+    c.a0 = k1;
+    c.a1 = k1 * k2 * -0.33332962f;
+    c.a2 = k1 * k2 * k2 * 0.13312598f;
+    c.a3 = k1 * k2 * k2 * k2 * -0.050222438f;
+    c.k2 = 2.f * LOG2E * kx;
+    c.lim = CAP_POLY_MAX / kx;
+    return c;
+}
+
+// One block of 32 rows x 32 columns of scores, 16 of them in a lane: distance (key - query position) of register r is  rel + SGN reg_off(r).
+//   z[r]: capped score, t[r]: z plus the part of the bias that differs between registers, c: the part that does not (per lane); log2 domain.
+//   lo: smallest distance of the block's first row to its columns, so that the block spans distances lo - 31 .. lo + 31
+template <int BIAS, bool CAP, int SGN> struct Scorer {
+    float sc2; Cap cp;
+    float sl2, rc[16];                       // BIAS 1: slope log2(e), and times reg_off(r)
+    const float* lut; int R; float far_lo, far_hi;
+    __device__ __forceinline__ void init(const PAArgs& p, float slope) {
+        sc2 = p.scale * LOG2E;
+        if (CAP) cp = cap_of(p.scale, p.cap);
+        if (BIAS == 1) {
+            sl2 = uniform_f(slope * LOG2E);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) rc[r] = uniform_f(sl2 * (float)reg_off(r));
+        }
+    }
+    __device__ __forceinline__ void block(f32x16& z, float (&t)[16], float& c, int rel, int lo) const {
+        if (CAP) {
+            float a = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) a = fmaxf(fmaxf(fabsf(z[r]), fabsf(z[r + 1])), a);
+            if (wave_all(a <= cp.lim)) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const float w = z[r] * z[r];
+                    z[r] *= fmaf(fmaf(fmaf(w, cp.a3, cp.a2), w, cp.a1), w, cp.a0);
+                }
+            } else {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) z[r] = fmaf(-2.f * cp.out, fast_rcp(fast_exp2(z[r] * cp.k2) + 1.f), cp.out);
+            }
+        }
+        c = 0.f;
+        const float f = CAP ? 1.f : sc2;
+        if (BIAS == 0) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) t[r] = z[r] * f;
+        } else if (BIAS == 1) {
+            if (lo + 31 <= 0) {
+                c = sl2 * (float)rel;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) t[r] = fmaf(z[r], f, SGN * rc[r]);
+            } else if (lo - 31 >= 0) {
+                c = -sl2 * (float)rel;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) t[r] = fmaf(z[r], f, -SGN * rc[r]);
+            } else {
+                const float d = (float)rel;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) t[r] = fmaf(-sl2, fabsf(d + (float)(SGN * reg_off(r))), z[r] * f);
+            }
+        } else {
+            if (lo + 31 <= -R || lo - 31 >= R) {
+                c = lo < 0 ? far_lo : far_hi;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) t[r] = z[r] * f;
+            } else {
+                const float* l = lut + PADL + R + rel;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) t[r] = fmaf(z[r], f, l[SGN * reg_off(r)]);
+            }
+        }
+    }
+};
+
+// distance -> learned bias of one head (log2 domain), clamped at the reach; entry PADL + R + distance
+__device__ __forceinline__ void load_lut(const PAArgs& p, int h, float* lut) {
+    for (int i = threadIdx.x; i < 2 * p.R + 1 + 2 * PADL; i += blockDim.x) {
+        const int b = clampi(p.buckets[clampi(i - PADL, 0, 2 * p.R)], 0, p.nbuckets - 1);
+        lut[i] = p.table[(long)b * p.H + h] * LOG2E;
+    }
+}
+
+// one operand row's four fragments (columns 16 ks + 8 hi .. + 7), zeros for a row outside
+__device__ __forceinline__ void row_frags(bf16x8 (&f)[4], const bf16_t* row, bool in, int hi) {
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) f[ks] = in ? ld<bf16x8>(row + ks * 16 + hi * 8) : bf16x8{0, 0, 0, 0, 0, 0, 0, 0};
+}
+
+// LDS-DMA of 64 rows each of two operands into a ring stage (K-type images: LDS row r holds tile row swap23(r)); rows beyond `last` read row
+// `last` (masked by the caller).  Wave-uniform 64-bit bases, 32-bit lane offsets: strides < 2^23 elements keep row * stride inside 24 x 24 bits
+struct Stager {
+    int row0; unsigned col0, s0, s1;          // byte strides
+    int wave;
+    __device__ __forceinline__ void init(int wave_, int lane, long st0, long st1) {
+        wave = wave_;
+        row0 = swap23(wave * 16 + (lane >> 3));
+        col0 = (unsigned)(((lane & 7) ^ swz(wave * 16 + (lane >> 3))) * 16);
+        s0 = (unsigned)(st0 * 2);
+        s1 = (unsigned)(st1 * 2);
+    }
+    __device__ __forceinline__ void issue(const bf16_t* a, const bf16_t* b, int last, unsigned char* S) const {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const unsigned row = (unsigned)min(row0 + 4 * u, last), col = col0 ^ (64u * u);
+            glds16((const char*)a + ((row & 0xffffffu) * (s0 & 0xffffffu) + col), S + (wave * 2 + u) * 1024);
+            glds16((const char*)b + ((row & 0xffffffu) * (s1 & 0xffffffu) + col), S + 8192 + (wave * 2 + u) * 1024);
+        }
+    }
+};
+
+// transposed fragments of a block (32 tile rows at T): f[s2][db] = columns 32 db + l31, rows 16 s2 + 8 hi .. + 7
+__device__ __forceinline__ void tr_frags(bf16x8 (&f)[2][2], const unsigned char* T, const TrOff& t) {
+    s16x4_ d[8];
+    lds_tr_read8<2048>(d, T + t.lo[0], T + t.hi_[0], T + t.lo[1], T + t.hi_[1]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i >> 1][i & 1] = __builtin_shufflevector(d[2 * i], d[2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+__device__ __forceinline__ f32x16 zero16() {
+    f32x16 z;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z[r] = 0.f;
+    return z;
+}
+
+// ------------------------------------------------------------------------------------------------ forward
+
+// One workgroup = 128 queries of one (document, head): 4 waves x 32; K / V tiles of 64 keys through a 2-stage LDS-DMA ring (the next tile in
+// flight while this one is computed, one raw barrier a tile).
+// TR: 0 inference, 1 training (log-sum-exps), 2 training with the table's gradient to come (two-term probabilities, o_lo)
+template <int BIAS, bool CAP, int TR>
+__global__ __launch_bounds__(256, 4) void pa_fwd_kernel(PAArgs p) {
+    __shared__ __attribute__((aligned(16))) unsigned char smem[2 * STAGE];
+    __shared__ float lut[BIAS == 2 ? 2 * REACH_MAX + 1 + 2 * PADL : 1];
+    lds_declare(smem, sizeof(smem));
+    if ((int)blockIdx.x >= p.nwork) {
+        fill_gap(p.cu_q, p.len_q, p.nd, p.Tq, p.O, p.so, p.ho, p.H, (int)blockIdx.x - p.nwork);
+        return;
+    }
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform_i(tid >> 6);
+    const int l31 = lane & 31, hi = lane >> 5;
+    const Work wk = work_of(p);
+    const int h = wk.h;
+    const Doc D = doc_of(p, wk.d);
+    if (wk.tile * 128 >= D.nq) return;
+    Scorer<BIAS, CAP, 1> sc;
+    sc.init(p, BIAS == 1 ? p.slopes[h] : 0.f);
+    if (BIAS == 2) {
+        load_lut(p, h, lut);
+        __syncthreads();
+        sc.lut = lut;
+        sc.R = p.R;
+        sc.far_lo = lut[PADL];
+        sc.far_hi = lut[PADL + 2 * p.R];
+    }
+    Stager sg;
+    sg.init(wave, lane, p.sk, p.sv);
+    int foff[4];
+    frag_offsets(l31, hi, foff);
+    const TrOff tro = tr_offsets(lane);
+    const bf16_t* Kb = p.K + (long)D.k0 * p.sk + (long)(h / p.G) * p.hk;
+    const bf16_t* Vb = p.V + (long)D.k0 * p.sv + (long)(h / p.G) * p.hv;
+
+    for (int tile = wk.tile; tile * 128 < D.nq; tile += p.nt) {
+        const int q0 = tile * 128 + wave * 32, q = q0 + l31;
+        const bool live = q0 < D.nq, qin = q < D.nq;
+        const int lim = qin ? D.lim(q) : 0;
+        const int lim_lo = live ? D.lim(q0) : 0, lim_hi = live ? D.lim(min(q0 + 31, D.nq - 1)) : 0;
+        const int kend = D.lim(min(tile * 128 + 127, D.nq - 1)), nt = (kend + 63) / 64;
+        bf16x8 qf[4];
+        row_frags(qf, p.Q + (long)(D.q0 + (qin ? q : 0)) * p.sq + (long)h * p.hq, qin, hi);
+        f32x16 o[2] = {zero16(), zero16()};
+        float m = M_INIT, l0 = 0.f, l1 = 0.f;
+        // (every ordinary load of the prologue is waited for before the first LDS-DMA: vmcnt is counted in order)
+        asm volatile("" ::"v"(qf[0]), "v"(qf[1]), "v"(qf[2]), "v"(qf[3]));
+        if (nt > 0) sg.issue(Kb, Vb, D.nk - 1, smem);
+        for (int kt = 0; kt < nt; ++kt) {
+            const int k0 = kt * 64;
+            wait_vmcnt<0>();              // tile kt has landed for this wave ...
+            barrier_raw();                // ... and for every wave; everyone is done with tile kt - 1
+            if (kt + 1 < nt) sg.issue(Kb + (long)(k0 + 64) * p.sk, Vb + (long)(k0 + 64) * p.sv, D.nk - 1 - (k0 + 64), smem + ((kt + 1) & 1) * STAGE);
+            const unsigned char* Kt = smem + (kt & 1) * STAGE;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                const int kk = k0 + 32 * kb;
+                if (kk >= lim_hi) continue;                   // (wave-uniform) nothing of the block is visible
+                f32x16 s = zero16();
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) s = mfma32(ld<bf16x8>(Kt + foff[ks] + kb * 4096), qf[ks], s);
+                float t[16], c;
+                const int qp = q0 + D.off;
+                sc.block(s, t, c, kk + 8 * hi - (qp + l31), kk - qp);
+                if (kk + 32 > lim_lo) {                       // some query of the wave does not see all of the block
+                    cold_path();
+                    const int n = lim - (kk + 8 * hi);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) t[r] = reg_off(r) < n ? t[r] : -__builtin_inff();
+                }
+                float mx = t[0];
+#pragma unroll
+                for (int r = 1; r < 16; ++r) mx = fmaxf(mx, t[r]);
+                mx += c;
+                if (!wave_all(mx <= m + M_SLACK)) {
+                    cold_path();
+                    const float mn = fmaxf(m, fmaxf(mx, lane32_other(mx))), al = fast_exp2(m - mn);
+                    l0 *= al;
+                    l1 *= al;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) { o[0][r] *= al; o[1][r] *= al; }
+                    m = mn;
+                }
+                const float mo = m - c;
+#pragma unroll
+                for (int r = 0; r < 16; r += 2) {
+                    t[r] = fast_exp2(t[r] - mo);
+                    t[r + 1] = fast_exp2(t[r + 1] - mo);
+                    l0 += t[r];
+                    l1 += t[r + 1];
+                }
+                const bf16x8 pf[2] = {pack8f(t), pack8f(t + 8)};
+                bf16x8 vf[2][2];
+                tr_frags(vf, Kt + 8192 + kb * 4096, tro);
+#pragma unroll
+                for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+                    for (int db = 0; db < 2; ++db) o[db] = mfma32(vf[s2][db], pf[s2], o[db]);
+                if (TR == 2) {
+#pragma unroll
+                    for (int s2 = 0; s2 < 2; ++s2) {
+                        float w[8];
+                        unpack8(__builtin_bit_cast(u32x4, pf[s2]), w);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) w[e] = t[8 * s2 + e] - w[e];
+                        const bf16x8 pl = pack8f(w);
+#pragma unroll
+                        for (int db = 0; db < 2; ++db) o[db] = mfma32(vf[s2][db], pl, o[db]);
+                    }
+                }
+            }
+        }
+        if (live) {
+            float l = l0 + l1;
+            l += lane32_other(l);                             // a row's keys are split over lanes l and l + 32
+            const float inv = l == 0.f ? 0.f : 1.f / l;       // (NaN stays NaN)
+            const int row = D.q0 + (qin ? q : 0);
+            if (TR && qin && hi == 0) p.lse2[(long)h * p.Tq + row] = l == 0.f ? LSE_EMPTY : m + log2f(l);
+            bf16_t* orow = p.O + (long)row * p.so + (long)h * p.ho;
+            bf16_t* lrow = TR == 2 ? p.Olo + ((long)row * p.H + h) * DH : nullptr;
+            store_rows32(o, hi, qin, [&](int db, int g, int hi_, bool ok, const float* a, const float* b) __attribute__((always_inline)) {
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { v[e] = a[e] * inv; v[4 + e] = b[e] * inv; }
+                u32x2 x = pack4(v), y = pack4(v + 4), xl, yl;
+                if (TR == 2) {
+                    float w[8], lo[8];
+                    unpack4(x, w);
+                    unpack4(y, w + 4);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) lo[e] = v[e] - w[e];
+                    xl = pack4(lo);
+                    yl = pack4(lo + 4);
+                    swap_pair(xl, yl);
+                }
+                swap_pair(x, y);
+                const int col = 32 * db + 8 * (g + hi_);
+                if (ok) {
+                    st<u32x4>(orow + col, u32x4{x[0], x[1], y[0], y[1]});
+                    if (TR == 2) st<u32x4>(lrow + col, u32x4{xl[0], xl[1], yl[0], yl[1]});
+                }
+            });
+        }
+        if ((tile + p.nt) * 128 < D.nq) __syncthreads();         // (another round: the ring is free again)
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ backward: dQ, dO.o, sums of dS by distance
+
+// sums of one block's dS (16 of them in a lane: query l31, keys reg_off(r) + 8 hi) along its diagonals, added to `dist` (entry = distance +
+// an offset folded into `base`).  The block goes through a wave's own LDS scratch ([16 keys][33]) in two halves; lane t (of 32) collects the
+// diagonals t and t - 32, whose elements are one per key: the scratch is read without bank conflicts, every distance has one owner, and the
+// order of the additions is fixed.
+__device__ __forceinline__ void diag_add(const float (&ds)[16], float* scr, float* dist_at_lo, int l31, int hi) {
+    float A = 0.f, B = 0.f;
+#pragma unroll
+    for (int s2 = 0; s2 < 2; ++s2) {
+        wave_sync();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) scr[(8 * hi + e) * 33 + l31] = ds[8 * s2 + e];
+        wave_sync();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int key = 16 * s2 + 8 * hi + j;               // half `hi` of the wave takes its eight keys of the sixteen
+            const int i = key - l31;                            // query of diagonal l31, or (wrapped) of diagonal l31 - 32
+            const float v = scr[(8 * hi + j) * 33 + (i & 31)];
+            A += i >= 0 ? v : 0.f;
+            B += i >= 0 ? 0.f : v;
+        }
+    }
+    A += lane32_other(A);
+    B += lane32_other(B);
+    // diagonals l31 (lower half-wave) and l31 - 32 (upper): 64 entries, each lane its own; dist_at_lo = entry of distance `lo`
+    dist_at_lo[hi ? l31 - 32 : l31] += hi ? B : A;
+}
+
+constexpr int distn(int reach) { return 2 * reach + 1 + 2 * PADL; }
+
+// RG: 0 no table gradient, else the largest reach of this instantiation (its LDS)
+template <int BIAS, bool CAP, int RG>
+__global__ __launch_bounds__(256, RG > 128 ? 2 : 3) void pa_dq_kernel(PAArgs p) {
+    __shared__ __attribute__((aligned(16))) unsigned char smem[2 * STAGE];
+    __shared__ float lut[BIAS == 2 ? distn(RG && RG < REACH_MAX ? RG : REACH_MAX) : 1];
+    __shared__ float dist[RG ? 4 * distn(RG) : 1];
+    __shared__ float scr[RG ? 4 * 16 * 33 : 1];
+    lds_declare(smem, sizeof(smem));
+    if ((int)blockIdx.x >= p.nwork) {
+        fill_gap(p.cu_q, p.len_q, p.nd, p.Tq, p.dQ, (long)p.H * DH, DH, p.H, (int)blockIdx.x - p.nwork);
+        return;
+    }
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform_i(tid >> 6);
+    const int l31 = lane & 31, hi = lane >> 5;
+    const Work wk = work_of(p);
+    const int h = wk.h;
+    const Doc D = doc_of(p, wk.d);
+    if (wk.tile * 128 >= D.nq) return;
+    const int ND = 2 * p.R + 1 + 2 * PADL;
+    Scorer<BIAS, CAP, 1> sc;
+    sc.init(p, BIAS == 1 ? p.slopes[h] : 0.f);
+    if (BIAS == 2) {
+        load_lut(p, h, lut);
+        if (RG) for (int i = tid; i < 4 * ND; i += 256) dist[i] = 0.f;
+        __syncthreads();
+        sc.lut = lut;
+        sc.R = p.R;
+        sc.far_lo = lut[PADL];
+        sc.far_hi = lut[PADL + 2 * p.R];
+    }
+    float* const mydist = dist + (RG ? wave * ND : 0);
+    float* const myscr = scr + (RG ? wave * 16 * 33 : 0);
+    float far_lo = 0.f, far_hi = 0.f;
+    const float icl = CAP ? 1.f / (p.cap * LOG2E) : 0.f;
+    Stager sg;
+    sg.init(wave, lane, p.sk, p.sv);
+    int foff[4];
+    frag_offsets(l31, hi, foff);
+    const TrOff tro = tr_offsets(lane);
+    const bf16_t* Kb = p.K + (long)D.k0 * p.sk + (long)(h / p.G) * p.hk;
+    const bf16_t* Vb = p.V + (long)D.k0 * p.sv + (long)(h / p.G) * p.hv;
+
+    for (int tile = wk.tile; tile * 128 < D.nq; tile += p.nt) {
+        const int q0 = tile * 128 + wave * 32, q = q0 + l31;
+        const bool live = q0 < D.nq, qin = q < D.nq;
+        const int lim = qin ? D.lim(q) : 0;
+        const int lim_lo = live ? D.lim(q0) : 0, lim_hi = live ? D.lim(min(q0 + 31, D.nq - 1)) : 0;
+        const int kend = D.lim(min(tile * 128 + 127, D.nq - 1)), nt = (kend + 63) / 64;
+        const int row = D.q0 + (qin ? q : 0);
+        bf16x8 qf[4], dof[4];
+        row_frags(qf, p.Q + (long)row * p.sq + (long)h * p.hq, qin, hi);
+        row_frags(dof, p.dO + (long)row * p.sg + (long)h * p.hg, qin, hi);
+        float dl = 0.f;
+        {
+            const bf16_t* orow = p.O + (long)row * p.so + (long)h * p.ho + hi * 8;
+            const bf16_t* lrow = p.Olo + ((long)row * p.H + h) * DH + hi * 8;
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+                float a[8], b[8], g[8];
+                unpack8(ld<u32x4>(orow + ks * 16), a);
+                if (RG) unpack8(ld<u32x4>(lrow + ks * 16), b);
+                unpack8(__builtin_bit_cast(u32x4, dof[ks]), g);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) dl = fmaf(g[e], RG ? a[e] + b[e] : a[e], dl);
+            }
+            dl += lane32_other(dl);
+            if (qin && hi == 0) p.delta[(long)h * p.Tq + row] = dl;
+        }
+        const float lse = qin ? p.lse2[(long)h * p.Tq + row] : LSE_EMPTY;
+        if (!qin) dl = 0.f;
+        f32x16 dq[2] = {zero16(), zero16()};
+        asm volatile("" ::"v"(qf[0]), "v"(qf[1]), "v"(qf[2]), "v"(qf[3]), "v"(dof[0]), "v"(dof[1]), "v"(dof[2]), "v"(dof[3]), "v"(lse), "v"(dl));
+        if (nt > 0) sg.issue(Kb, Vb, D.nk - 1, smem);
+        for (int kt = 0; kt < nt; ++kt) {
+            const int k0 = kt * 64;
+            wait_vmcnt<0>();
+            barrier_raw();
+            if (kt + 1 < nt) sg.issue(Kb + (long)(k0 + 64) * p.sk, Vb + (long)(k0 + 64) * p.sv, D.nk - 1 - (k0 + 64), smem + ((kt + 1) & 1) * STAGE);
+            const unsigned char* Kt = smem + (kt & 1) * STAGE;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                const int kk = k0 + 32 * kb;
+                if (kk >= lim_hi) continue;
+                f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) {
+                    s = mfma32(ld<bf16x8>(Kt + foff[ks] + kb * 4096), qf[ks], s);
+                    dp = mfma32(ld<bf16x8>(Kt + 8192 + foff[ks] + kb * 4096), dof[ks], dp);
+                }
+                float t[16], c;
+                const int qp = q0 + D.off, lo = kk - qp;
+                sc.block(s, t, c, kk + 8 * hi - (qp + l31), lo);
+                if (kk + 32 > lim_lo) {
+                    cold_path();
+                    const int n = lim - (kk + 8 * hi);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) t[r] = reg_off(r) < n ? t[r] : -__builtin_inff();
+                }
+                const float mo = lse - c;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) t[r] = fast_exp2(t[r] - mo) * (dp[r] - dl);       // dS
+                if (RG) {
+                    if (lo + 31 <= -p.R || lo - 31 >= p.R) {
+                        float a = 0.f;
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) a += t[r];
+                        if (lo < 0) far_lo += a; else far_hi += a;
+                    } else {
+                        diag_add(t, myscr, mydist + PADL + p.R + lo, l31, hi);
+                    }
+                }
+                if (CAP) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const float th = s[r] * icl;
+                        t[r] *= fmaf(-th, th, 1.f);
+                    }
+                }
+                const bf16x8 df[2] = {pack8f(t), pack8f(t + 8)};
+                bf16x8 kf[2][2];
+                tr_frags(kf, Kt + kb * 4096, tro);
+#pragma unroll
+                for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+                    for (int db = 0; db < 2; ++db) dq[db] = mfma32(kf[s2][db], df[s2], dq[db]);
+            }
+        }
+        if (live) {
+            bf16_t* drow = p.dQ + ((long)row * p.H + h) * DH;
+            store_rows32(dq, hi, qin, [&](int db, int g, int hi_, bool ok, const float* a, const float* b) __attribute__((always_inline)) {
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { v[e] = a[e] * p.scale; v[4 + e] = b[e] * p.scale; }
+                u32x2 x = pack4(v), y = pack4(v + 4);
+                swap_pair(x, y);
+                if (ok) st<u32x4>(drow + 32 * db + 8 * (g + hi_), u32x4{x[0], x[1], y[0], y[1]});
+            });
+        }
+        if ((tile + p.nt) * 128 < D.nq) __syncthreads();
+    }
+    if (RG) {
+        // sums by distance, clamped at the reach: entries beyond it join the ends, with the far blocks' sums; four waves in order
+        far_lo = wave_sum_fast(far_lo);
+        far_hi = wave_sum_fast(far_hi);
+        wave_sync();
+        float a = lane < PADL ? mydist[lane] : 0.f, b = lane < PADL ? mydist[PADL + 2 * p.R + 1 + lane] : 0.f;
+        a = wave_sum_fast(a);
+        b = wave_sum_fast(b);
+        wave_sync();
+        if (lane == 0) {
+            mydist[PADL] += far_lo + a;
+            mydist[PADL + 2 * p.R] += far_hi + b;
+        }
+        __syncthreads();
+        float* out = p.dist + (long)wk.lin * (2 * p.R + 1);
+        for (int i = tid; i < 2 * p.R + 1; i += 256) {
+            const float* d = dist + PADL + i;
+            out[i] = (d[0] + d[ND]) + (d[2 * ND] + d[3 * ND]);
+        }
+    }
+}
+
+// sums over the workgroups of a head -> by_dist[h][2 R + 1]; 64 distances x 16 row groups per workgroup
+__global__ __launch_bounds__(1024) void pa_dist_reduce_kernel(PAArgs p, float* by_dist) {
+    __shared__ float sm[16][64];
+    const int lane = threadIdx.x & 63, grp = threadIdx.x >> 6, h = blockIdx.y;
+    const int N = 2 * p.R + 1, i = blockIdx.x * 64 + lane;
+    float a = 0.f;
+    const float* q = p.dist + (long)h * p.nd * p.nt * N + i;
+#pragma unroll 4
+    for (int w = grp; w < p.nd * p.nt; w += 16) {
+        const int t = p.nt - 1 - w % p.nt;                        // (Work::tile of this row of partial sums)
+        if (i < N && t * 128 < span(p.cu_q, p.len_q, w / p.nt, p.Tq).n) a += q[(long)w * N];
+    }
+    sm[grp][lane] = a;
+    __syncthreads();
+    if (grp == 0 && i < N) {
+        a = 0.f;
+#pragma unroll
+        for (int g = 0; g < 16; ++g) a += sm[g][lane];
+        by_dist[(long)h * N + i] = a;
+    }
+}
+// sums over the distances of a bucket -> dtable[bucket][h]; one wave each
+__global__ __launch_bounds__(256) void pa_table_grad_kernel(const float* by_dist, const int* buckets, int N, int nbuckets, int H, float* dtable, int accumulate) {
+    const int lane = threadIdx.x & 63, w = blockIdx.x * 4 + uniform_i(threadIdx.x >> 6);
+    if (w >= nbuckets * H) return;
+    const int b = w / H, h = w % H;
+    float a = 0.f;
+    for (int i = lane; i < N; i += 64) a += clampi(buckets[i], 0, nbuckets - 1) == b ? by_dist[(long)h * N + i] : 0.f;
+    a = wave_sum_fast(a);
+    if (lane == 0) dtable[w] = accumulate ? dtable[w] + a : a;
+}
+
+// ------------------------------------------------------------------------------------------------ backward: dK, dV
+
+// One workgroup = 128 keys of one (document, key head); sweep over the 64-query tiles of all its query heads.  The query rows of the Q / dO tiles
+// are K-type images, so the accumulators (rows = queries) are the B operands of dV^T = dO^T P and dK^T = Q^T dS; their A operands come out of the
+// same tiles by transposing reads.  The 64 lse / delta values of a query tile ride along in the ring stage.
+constexpr int KSTAGE = STAGE + 512;
+
+template <int BIAS, bool CAP>
+__global__ __launch_bounds__(256, 2) void pa_dkv_kernel(PAArgs p) {
+    __shared__ __attribute__((aligned(16))) unsigned char smem[2 * KSTAGE];
+    __shared__ float lut[BIAS == 2 ? 2 * distn(REACH_MAX) : 1];        // two heads' tables in turn
+    lds_declare(smem, sizeof(smem));
+    if ((int)blockIdx.x >= p.nwork) {
+        fill_gap(p.cu_k, p.len_k, p.nd, p.Tk, p.dK, (long)p.Hkv * DH, DH, p.Hkv, (int)blockIdx.x - p.nwork);
+        fill_gap(p.cu_k, p.len_k, p.nd, p.Tk, p.dV, (long)p.Hkv * DH, DH, p.Hkv, (int)blockIdx.x - p.nwork);
+        return;
+    }
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform_i(tid >> 6);
+    const int l31 = lane & 31, hi = lane >> 5;
+    const Work wk = work_of(p);
+    const Doc D = doc_of(p, wk.d);
+    const int tile0 = p.nt - 1 - wk.tile;          // (causal: the first keys are seen by the most queries)
+    if (tile0 * 128 >= D.nk) return;
+    Stager sg;
+    sg.init(wave, lane, p.sq, p.sg);
+    int foff[4];
+    frag_offsets(l31, hi, foff);
+    const TrOff tro = tr_offsets(lane);
+    const float icl = CAP ? 1.f / (p.cap * LOG2E) : 0.f;
+    const int nqt = (D.nq + 63) / 64;
+
+    for (int tile = tile0; tile * 128 < D.nk; tile += p.nt) {
+        const int kk = tile * 128 + wave * 32, key = kk + l31;
+        const bool live = kk < D.nk, kin = key < D.nk;
+        bf16x8 kf[4], vf[4];
+        row_frags(kf, p.K + (long)(D.k0 + (kin ? key : 0)) * p.sk + (long)wk.h * p.hk, kin, hi);
+        row_frags(vf, p.V + (long)(D.k0 + (kin ? key : 0)) * p.sv + (long)wk.h * p.hv, kin, hi);
+        f32x16 dk[2] = {zero16(), zero16()}, dv[2] = {zero16(), zero16()};
+        // first query that sees this lane's key, and the first query tile that sees any key of the workgroup
+        const int qmin = (!D.causal || key < D.prefix) ? -0x40000000 : key - D.off;
+        int t0 = 0;
+        if (D.causal && tile * 128 >= D.prefix) t0 = max(0, tile * 128 - D.off) / 64;
+        const int per = max(0, nqt - t0), total = per * p.G;
+        int ih = 0, iq = 0, ch = 0, cq = 0;          // head and tile that is fetched / computed next
+        auto issue = [&](int it) __attribute__((always_inline)) {
+            const int h = wk.h * p.G + ih, q0 = (t0 + iq) * 64;
+            if (++iq == per) { iq = 0; ++ih; }
+            unsigned char* S = smem + (it & 1) * KSTAGE;
+            const long r = D.q0 + q0;
+            sg.issue(p.Q + r * p.sq + (long)h * p.hq, p.dO + r * p.sg + (long)h * p.hg, D.nq - 1 - q0, S);
+            if (wave < 2) glds4((wave == 0 ? p.lse2 : p.delta) + (long)h * p.Tq + r + min(lane, D.nq - 1 - q0), S + STAGE + wave * 256);
+        };
+        Scorer<BIAS, CAP, -1> sc;
+        sc.init(p, BIAS == 1 ? p.slopes[wk.h * p.G] : 0.f);
+        if (BIAS == 2) {
+            sc.R = p.R;
+            if (total > 0) load_lut(p, wk.h * p.G, lut);
+            wait_lgkm0();
+        }
+        asm volatile("" ::"v"(kf[0]), "v"(kf[1]), "v"(kf[2]), "v"(kf[3]), "v"(vf[0]), "v"(vf[1]), "v"(vf[2]), "v"(vf[3]));
+        if (total > 0) issue(0);
+        for (int it = 0; it < total; ++it) {
+            const int hd = ch, j0 = cq, q0 = (t0 + j0) * 64;
+            if (++cq == per) { cq = 0; ++ch; }
+            wait_vmcnt<0>();
+            barrier_raw();
+            if (it + 1 < total) issue(it + 1);
+            if (BIAS == 1 && p.G > 1 && j0 == 0 && hd > 0) sc.init(p, p.slopes[wk.h * p.G + hd]);
+            if (BIAS == 2) {
+                float* L = lut + (hd & 1) * distn(REACH_MAX);
+                sc.lut = L;
+                sc.far_lo = L[PADL];
+                sc.far_hi = L[PADL + 2 * p.R];
+                // the next head's table while this head's last tile is computed (the other buffer: its last reader passed the barrier above)
+                if (j0 == per - 1 && hd + 1 < p.G) {
+                    load_lut(p, wk.h * p.G + hd + 1, lut + ((hd + 1) & 1) * distn(REACH_MAX));
+                    wait_lgkm0();
+                }
+            }
+            if (!live) continue;
+            const unsigned char* Qt = smem + (it & 1) * KSTAGE;
+            const float* lse_s = (const float*)(Qt + STAGE);
+#pragma unroll
+            for (int qb = 0; qb < 2; ++qb) {
+                const int qq = q0 + 32 * qb;                  // first query of the block
+                if (qq >= D.nq || D.lim(min(qq + 31, D.nq - 1)) <= kk) continue;
+                f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) {
+                    s = mfma32(ld<bf16x8>(Qt + foff[ks] + qb * 4096), kf[ks], s);
+                    dp = mfma32(ld<bf16x8>(Qt + 8192 + foff[ks] + qb * 4096), vf[ks], dp);
+                }
+                float t[16], c;
+                const int qp = qq + D.off;
+                sc.block(s, t, c, key - (qp + 8 * hi), kk - qp);
+                if (D.lim(qq) < kk + 32 || qq + 32 > D.nq) {
+                    cold_path();
+                    const int a = qmin - (qq + 8 * hi), b = D.nq - (qq + 8 * hi);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) t[r] = (reg_off(r) >= a && reg_off(r) < b) ? t[r] : -__builtin_inff();
+                }
+                const float* ls = lse_s + 32 * qb + 8 * hi;
+                float ds[16];
+#pragma unroll
+                for (int r4 = 0; r4 < 16; r4 += 4) {
+                    const f32x4 l4 = ld<f32x4>(ls + reg_off(r4)), d4 = ld<f32x4>(ls + 64 + reg_off(r4));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int r = r4 + j;
+                        t[r] = fast_exp2(t[r] - (BIAS == 0 ? l4[j] : l4[j] - c));
+                        ds[r] = t[r] * (dp[r] - d4[j]);
+                        if (CAP) {
+                            const float th = s[r] * icl;
+                            ds[r] *= fmaf(-th, th, 1.f);
+                        }
+                    }
+                }
+                bf16x8 f[2][2];
+                tr_frags(f, Qt + 8192 + qb * 4096, tro);
+                const bf16x8 pf[2] = {pack8f(t), pack8f(t + 8)};
+#pragma unroll
+                for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+                    for (int db = 0; db < 2; ++db) dv[db] = mfma32(f[s2][db], pf[s2], dv[db]);
+                tr_frags(f, Qt + qb * 4096, tro);
+                const bf16x8 df[2] = {pack8f(ds), pack8f(ds + 8)};
+#pragma unroll
+                for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+                    for (int db = 0; db < 2; ++db) dk[db] = mfma32(f[s2][db], df[s2], dk[db]);
+            }
+        }
+        if (live) {
+            const long orow = ((long)(D.k0 + (kin ? key : 0)) * p.Hkv + wk.h) * DH;
+            auto put = [&](bf16_t* dst, float f, int db, int g, int hi_, bool ok, const float* a, const float* b) __attribute__((always_inline)) {
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { v[e] = a[e] * f; v[4 + e] = b[e] * f; }
+                u32x2 x = pack4(v), y = pack4(v + 4);
+                swap_pair(x, y);
+                if (ok) st<u32x4>(dst + orow + 32 * db + 8 * (g + hi_), u32x4{x[0], x[1], y[0], y[1]});
+            };
+            store_rows32(dk, hi, kin, [&](int db, int g, int hi_, bool ok, const float* a, const float* b) __attribute__((always_inline)) { put(p.dK, p.scale, db, g, hi_, ok, a, b); });
+            store_rows32(dv, hi, kin, [&](int db, int g, int hi_, bool ok, const float* a, const float* b) __attribute__((always_inline)) { put(p.dV, 1.f, db, g, hi_, ok, a, b); });
+        }
+        if ((tile + p.nt) * 128 < D.nk) __syncthreads();
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+bool strides_ok(long t, long h) { return t % 8 == 0 && h % 8 == 0 && t >= 0 && h >= 0 && t < (1 << 23); }
+
+// sizes, pointers and layouts that the kernels assume
+int check(const PAArgs& a) {
+    if (a.nd < 0 || a.Tq < 0 || a.Tk < 0 || a.H < 1 || a.Hkv < 1 || a.H % a.Hkv != 0) return E2K_ERR_SHAPE;
+    if (a.nd > 0 && (!a.cu_q || !a.cu_k)) return E2K_ERR_ARG;
+    if (!(a.scale > 0.f) || !(a.cap >= 0.f) || !(a.scale < 1e30f) || !(a.cap < 1e30f)) return E2K_ERR_ARG;
+    if (a.slopes && a.table) return E2K_ERR_ARG;
+    if (a.table && (!a.buckets || a.nbuckets < 1 || a.R < 0 || a.R > REACH_MAX)) return E2K_ERR_SHAPE;
+    if (!a.Q || (a.Tk > 0 && (!a.K || !a.V))) return E2K_ERR_ARG;
+    if (!strides_ok(a.sq, a.hq) || !strides_ok(a.sk, a.hk) || !strides_ok(a.sv, a.hv) || !strides_ok(a.so, a.ho)) return E2K_ERR_ALIGN;
+    if (!aligned16(a.Q) || !aligned16(a.K) || !aligned16(a.V) || !aligned16(a.O)) return E2K_ERR_ALIGN;
+    return E2K_OK;
+}
+// grid of `rows`-row problems: tiles per (document, head) and workgroups
+int plan_grid(PAArgs& a, int longest, int total, int heads, long& grid) {
+    if (longest <= 0 || longest > total) longest = total;
+    a.nt = (longest + 127) / 128;
+    if (a.nt < 1) a.nt = 1;
+    const long work = (long)a.nd * a.nt * heads;
+    grid = work + (a.fill ? (long)(a.nd + 1) * GAP_PARTS : 0);
+    if (grid > 0x7fffffffL / 256) return E2K_ERR_SHAPE;
+    a.nwork = (int)work;
+    return E2K_OK;
+}
+
+template <int BIAS, bool CAP> void run_fwd(const PAArgs& a, int train, long grid, hipStream_t st) {
+    if (BIAS == 2 && train == 2) hipLaunchKernelGGL((pa_fwd_kernel<BIAS, CAP, BIAS == 2 ? 2 : 1>), dim3((unsigned)grid), dim3(256), 0, st, a);
+    else if (train) hipLaunchKernelGGL((pa_fwd_kernel<BIAS, CAP, 1>), dim3((unsigned)grid), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((pa_fwd_kernel<BIAS, CAP, 0>), dim3((unsigned)grid), dim3(256), 0, st, a);
+}
+template <int BIAS, bool CAP> void run_dq(const PAArgs& a, int rg, long grid, hipStream_t st) {
+    if (BIAS == 2 && rg == 1) hipLaunchKernelGGL((pa_dq_kernel<BIAS, CAP, BIAS == 2 ? 128 : 0>), dim3((unsigned)grid), dim3(256), 0, st, a);
+    else if (BIAS == 2 && rg == 2) hipLaunchKernelGGL((pa_dq_kernel<BIAS, CAP, BIAS == 2 ? REACH_MAX : 0>), dim3((unsigned)grid), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((pa_dq_kernel<BIAS, CAP, 0>), dim3((unsigned)grid), dim3(256), 0, st, a);
+}
+template <int BIAS, bool CAP> void run_dkv(const PAArgs& a, int, long grid, hipStream_t st) {
+    hipLaunchKernelGGL((pa_dkv_kernel<BIAS, CAP>), dim3((unsigned)grid), dim3(256), 0, st, a);
+}
+#define PA_PICK(FN, a, ...)                                                                       \
+    do {                                                                                          \
+        const bool cap_ = (a).cap > 0.f;                                                          \
+        if ((a).table) { if (cap_) FN<2, true>(a, __VA_ARGS__); else FN<2, false>(a, __VA_ARGS__); }        \
+        else if ((a).slopes) { if (cap_) FN<1, true>(a, __VA_ARGS__); else FN<1, false>(a, __VA_ARGS__); }  \
+        else { if (cap_) FN<0, true>(a, __VA_ARGS__); else FN<0, false>(a, __VA_ARGS__); }                  \
+    } while (0)
+
+PAArgs common(const void* Q, int64_t sq, int64_t hq, const void* K, int64_t sk, int64_t hk, const void* V, int64_t sv, int64_t hv, const int32_t* cu_q,
+              const int32_t* cu_k, const int32_t* len_q, const int32_t* len_k, const int32_t* prefix, int nd, int Tq, int Tk, int H, int Hkv, int causal,
+              float scale, float softcap, const float* slopes, const float* table, const int32_t* buckets, int nbuckets, int reach) {
+    PAArgs a{};
+    a.Q = (const bf16_t*)Q; a.K = (const bf16_t*)K; a.V = (const bf16_t*)V;
+    a.sq = sq; a.hq = hq; a.sk = sk; a.hk = hk; a.sv = sv; a.hv = hv;
+    a.cu_q = cu_q; a.cu_k = cu_k; a.len_q = len_q; a.len_k = len_k; a.prefix = prefix;
+    a.nd = nd; a.Tq = Tq; a.Tk = Tk; a.H = H; a.Hkv = Hkv; a.G = Hkv > 0 ? H / Hkv : 1;
+    a.causal = causal; a.scale = scale; a.cap = softcap;
+    a.slopes = slopes; a.table = table; a.buckets = buckets; a.nbuckets = nbuckets; a.R = reach;
+    return a;
+}
+
+int packed_attn_fwd_impl(const void* Q, int64_t sq, int64_t hq, const void* K, int64_t sk, int64_t hk, const void* V, int64_t sv, int64_t hv,
+                         const int32_t* cu_q, const int32_t* cu_k, const int32_t* len_q, const int32_t* len_k, const int32_t* prefix, int nd, int Tq,
+                         int Tk, int H, int Hkv, int max_q, int causal, float scale, float softcap, const float* slopes, const float* table,
+                         const int32_t* buckets, int nbuckets, int reach, void* O, int64_t so, int64_t ho, void* Olo, float* lse2, int fill_gaps,
+                         void* stream) {
+    PAArgs a = common(Q, sq, hq, K, sk, hk, V, sv, hv, cu_q, cu_k, len_q, len_k, prefix, nd, Tq, Tk, H, Hkv, causal, scale, softcap, slopes, table,
+                      buckets, nbuckets, reach);
+    a.O = (bf16_t*)O; a.so = so; a.ho = ho; a.Olo = (bf16_t*)Olo; a.lse2 = lse2; a.fill = fill_gaps;
+    if (Tq == 0) return E2K_OK;
+    const int rc = check(a);
+    if (rc) return rc;
+    if (!O || (Olo && (!lse2 || !table))) return E2K_ERR_ARG;
+    if (!aligned16(Olo)) return E2K_ERR_ALIGN;
+    long grid;
+    const int rg = plan_grid(a, max_q, Tq, H, grid);
+    if (rg) return rg;
+    if (grid == 0) return E2K_OK;
+    hipStream_t st = (hipStream_t)stream;
+    PA_PICK(run_fwd, a, Olo ? 2 : lse2 ? 1 : 0, grid, st);
+    E2K_CHECK_LAUNCH();
+    return E2K_OK;
+}
+
+int packed_attn_bwd_impl(const void* dO, int64_t sg, int64_t hg, const void* Q, int64_t sq, int64_t hq, const void* K, int64_t sk, int64_t hk,
+                         const void* V, int64_t sv, int64_t hv, const int32_t* cu_q, const int32_t* cu_k, const int32_t* len_q, const int32_t* len_k,
+                         const int32_t* prefix, int nd, int Tq, int Tk, int H, int Hkv, int max_q, int max_k, int causal, float scale, float softcap,
+                         const float* slopes, const float* table, const int32_t* buckets, int nbuckets, int reach, const void* O, int64_t so, int64_t ho,
+                         const void* Olo, const float* lse2, float* delta, void* dQ, void* dK, void* dV, float* dtable, int accumulate, float* ws,
+                         int fill_gaps, void* stream) {
+    PAArgs a = common(Q, sq, hq, K, sk, hk, V, sv, hv, cu_q, cu_k, len_q, len_k, prefix, nd, Tq, Tk, H, Hkv, causal, scale, softcap, slopes, table,
+                      buckets, nbuckets, reach);
+    a.dO = (const bf16_t*)dO; a.sg = sg; a.hg = hg; a.O = (bf16_t*)O; a.so = so; a.ho = ho; a.Olo = (bf16_t*)Olo; a.lse2 = (float*)lse2; a.delta = delta;
+    a.dQ = (bf16_t*)dQ; a.dK = (bf16_t*)dK; a.dV = (bf16_t*)dV; a.dist = ws; a.fill = fill_gaps;
+    hipStream_t st = (hipStream_t)stream;
+    long grid;
+    if (Tq > 0) {
+        const int rc = check(a);
+        if (rc) return rc;
+        if (!dO || !O || !lse2 || !delta || !dQ || (dtable && (!table || !ws || !Olo))) return E2K_ERR_ARG;
+        if (!strides_ok(sg, hg) || !aligned16(dO) || !aligned16(Olo) || !aligned16(dQ) || !aligned16(dK) || !aligned16(dV)) return E2K_ERR_ALIGN;
+        if (Tk > 0 && (!dK || !dV)) return E2K_ERR_ARG;
+        const int rg = plan_grid(a, max_q, Tq, H, grid);
+        if (rg) return rg;
+        if (grid > 0) {
+            PA_PICK(run_dq, a, dtable ? (reach <= 128 ? 1 : 2) : 0, grid, st);
+            E2K_CHECK_LAUNCH();
+        }
+    } else if (nd < 0 || Tk < 0 || H < 1 || Hkv < 1 || H % Hkv != 0) {
+        return E2K_ERR_SHAPE;
+    }
+    if (dtable) {
+        if (!table || !ws || nbuckets < 1 || reach < 0 || reach > REACH_MAX) return E2K_ERR_ARG;
+        const int N = 2 * reach + 1;
+        float* by_dist = ws + (Tq > 0 ? (long)a.nwork * N : 0);
+        if (Tq == 0) a.nd = 0;                 // nothing was written: the sums are empty
+        hipLaunchKernelGGL(pa_dist_reduce_kernel, dim3((N + 63) / 64, H), dim3(1024), 0, st, a, by_dist);
+        E2K_CHECK_LAUNCH();
+        hipLaunchKernelGGL(pa_table_grad_kernel, dim3((nbuckets * H + 3) / 4), dim3(256), 0, st, by_dist, buckets, N, nbuckets, H, dtable, accumulate);
+        E2K_CHECK_LAUNCH();
+        a.nd = nd;
+    }
+    if (Tk > 0) {
+        if (!dK || !dV || !aligned16(dK) || !aligned16(dV)) return E2K_ERR_ARG;
+        const int rg = plan_grid(a, max_k, Tk, Hkv, grid);
+        if (rg) return rg;
+        if (grid > 0) {
+            PA_PICK(run_dkv, a, 0, grid, st);
+            E2K_CHECK_LAUNCH();
+        }
+    }
+    return E2K_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int e2k_packed_attn_fwd(const void* Q, int64_t sq, int64_t hq, const void* K, int64_t sk, int64_t hk, const void* V, int64_t sv, int64_t hv,
+                        const int32_t* cu_q, const int32_t* cu_k, const int32_t* len_q, const int32_t* len_k, const int32_t* prefix, int nd, int Tq,
+                        int Tk, int H, int Hkv, int max_q, int causal, float scale, float softcap, const float* slopes, const float* table,
+                        const int32_t* buckets, int nbuckets, int reach, void* O, int64_t so, int64_t ho, void* Olo, float* lse2, int fill_gaps,
+                        void* stream) {
+    return e2k::dispatch("packed_attn_fwd", packed_attn_fwd_impl, Q, sq, hq, K, sk, hk, V, sv, hv, cu_q, cu_k, len_q, len_k, prefix, nd, Tq, Tk, H, Hkv,
+                         max_q, causal, scale, softcap, slopes, table, buckets, nbuckets, reach, O, so, ho, Olo, lse2, fill_gaps, stream);
+}
+int64_t e2k_query_packed_attn_bwd_ws_floats(int nd, int Tq, int H, int max_q, int reach) {
+    if (nd < 0 || Tq < 0 || H < 1 || reach < 0 || reach > REACH_MAX) return 0;
+    if (max_q <= 0 || max_q > Tq) max_q = Tq;
+    const int64_t nt = max_q > 0 ? (max_q + 127) / 128 : 1;
+    return ((Tq > 0 ? nd * nt * H : 0) + H) * (2 * (int64_t)reach + 1);
+}
+int e2k_packed_attn_bwd(const void* dO, int64_t sg, int64_t hg, const void* Q, int64_t sq, int64_t hq, const void* K, int64_t sk, int64_t hk,
+                        const void* V, int64_t sv, int64_t hv, const int32_t* cu_q, const int32_t* cu_k, const int32_t* len_q, const int32_t* len_k,
+                        const int32_t* prefix, int nd, int Tq, int Tk, int H, int Hkv, int max_q, int max_k, int causal, float scale, float softcap,
+                        const float* slopes, const float* table, const int32_t* buckets, int nbuckets, int reach, const void* O, int64_t so, int64_t ho,
+                        const void* Olo, const float* lse2, float* delta, void* dQ, void* dK, void* dV, float* dtable, int accumulate, float* ws,
+                        int fill_gaps, void* stream) {
+    return e2k::dispatch("packed_attn_bwd", packed_attn_bwd_impl, dO, sg, hg, Q, sq, hq, K, sk, hk, V, sv, hv, cu_q, cu_k, len_q, len_k, prefix, nd, Tq,
+                         Tk, H, Hkv, max_q, max_k, causal, scale, softcap, slopes, table, buckets, nbuckets, reach, O, so, ho, Olo, lse2, delta, dQ, dK,
+                         dV, dtable, accumulate, ws, fill_gaps, stream);
+}
+
+}  // extern "C"

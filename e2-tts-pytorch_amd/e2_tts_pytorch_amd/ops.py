@@ -1021,6 +1021,181 @@ def qkv_post_bwd(st, dQ, dK, dV, dgate_pre, qkvg, cosb, sinb, vfirst=None, dvfir
     return dqkvg
 
 
+# ------------------------------------------------------------------------------------------------ attention over packed documents
+
+class _on_device:
+    """kernels launch on the device of their tensors, whichever is current"""
+    __slots__ = ('guard',)
+
+    def __init__(self, t):
+        self.guard = torch.cuda.device(t.device) if t.is_cuda and t.device.index != torch.cuda.current_device() else None
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+        return False
+
+
+def _heads64(t, what):
+    """(tokens, heads, 64) bf16 that the kernels can read in place (16-byte rows, strides they can address), a contiguous copy otherwise"""
+    if t.dim() != 3 or t.shape[2] != 64 or t.dtype != bf16:
+        raise E2KError(f'packed attention: {what} must be (tokens, heads, 64) bf16, got {t.dtype} {tuple(t.shape)}')
+    s0, s1, s2 = t.stride()
+    if s2 != 1 or s0 % 8 or s1 % 8 or s0 >= 1 << 23 or t.data_ptr() % 16:
+        t = t.contiguous()
+    return t
+
+
+def _offsets(cu, what, device, n=None):
+    if cu.dtype != torch.int32 or cu.dim() != 1 or not cu.is_contiguous() or cu.device != device or (cu.numel() != n if n is not None else cu.numel() < 1):
+        raise E2KError(f'packed attention: {what} must be contiguous int32 on the device of q' + (f', {n} of them' if n is not None else ''))
+    return cu
+
+
+def _score_args(H, device, scale, softcap, slopes, table, buckets, what='packed attention'):
+    """checks of the score's options -> (scale, softcap, number of buckets, reach)"""
+    scale = 0.125 if scale is None else float(scale)
+    softcap = float(softcap)
+    if not 0. < scale < 1e30 or not 0. <= softcap < 1e30:
+        raise E2KError(f'{what}: scale must be positive and softcap not negative, got {scale}, {softcap}')
+    if slopes is not None and table is not None:
+        raise E2KError(f'{what}: slopes or a table, not both')
+    if slopes is not None and (slopes.dtype != f32 or slopes.shape != (H,) or not slopes.is_contiguous() or slopes.device != device):
+        raise E2KError(f'{what}: slopes must be contiguous fp32 ({H},) on the device of q')
+    if (table is None) != (buckets is None):
+        raise E2KError(f'{what}: table and buckets go together')
+    if table is None:
+        return scale, softcap, 0, 0
+    if table.dtype != f32 or table.dim() != 2 or table.shape[1] != H or table.shape[0] < 1 or not table.is_contiguous() or table.device != device:
+        raise E2KError(f'{what}: table must be contiguous fp32 (buckets, {H}) on the device of q')
+    if buckets.dtype != torch.int32 or buckets.dim() != 1 or buckets.numel() % 2 != 1 or buckets.numel() > 1025 or not buckets.is_contiguous() or buckets.device != device:
+        raise E2KError(f'{what}: buckets must be contiguous int32 (2 reach + 1,), reach <= 512, on the device of q')
+    return scale, softcap, table.shape[0], buckets.numel() // 2
+
+
+def rel_buckets(num_buckets=32, max_distance=128, causal=False, device=None):
+    """bucket of every key - query distance -max_distance .. max_distance (int32), the T5 scheme: one bucket per distance up to half of a side's
+    buckets, then logarithmically wider ones, the last for max_distance and beyond; both sides have buckets of their own unless causal.  Borders
+    in whole numbers: n lies in the j-th wide bucket when (n / near)^far >= (max_distance / near)^j"""
+    side = num_buckets if causal else num_buckets // 2
+    near = side // 2
+    far = side - near
+    if near < 1 or not near < max_distance <= 512:
+        raise E2KError(f'rel_buckets: num_buckets {num_buckets} too few, or max_distance {max_distance} not between {near} and 512')
+    start = [near]                           # first distance of each wide bucket
+    for j in range(1, far):
+        n = start[-1]
+        while n ** far * near ** j < max_distance ** j * near ** far:
+            n += 1
+        start.append(n)
+    of = [n if n < near else near + sum(n >= s for s in start[1:]) for n in range(max_distance + 1)]
+    back = of[:0:-1]
+    ahead = [0] * max_distance if causal else [b + side for b in of[1:]]
+    return torch.tensor(back + [of[0]] + ahead, dtype=torch.int32, device=device)
+
+
+class PackedAttnState:
+    """what packed_attn_fwd(train=True) keeps for packed_attn_bwd"""
+    __slots__ = ('q', 'k', 'v', 'cu_q', 'cu_k', 'len_q', 'len_k', 'prefix', 'max_q', 'max_k', 'causal', 'scale', 'softcap', 'slopes', 'table', 'buckets',
+                 'reach', 'out', 'lo', 'lse2')
+
+
+def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, len_q=None, len_k=None, prefix=None, max_q=0, max_k=0, causal=False, scale=None, softcap=0., slopes=None,
+                    table=None, buckets=None, out=None, train=False, table_grad=True):
+    """Attention over documents that lie one behind the other: q (Tq,H,64), k / v (Tk,Hkv,64) bf16 with Hkv dividing H; document d has the query rows
+    cu_q[d]:cu_q[d+1] and the key rows cu_k[d]:cu_k[d+1] (int32 offsets on the device; cu_k None: the same as cu_q), only the first len_q[d] /
+    len_k[d] of them where given (int32).  causal: a query sees the keys up to its own position (the last query stands on the last key) and the first
+    prefix[d] keys.  softcap > 0: scores capped to softcap * tanh(score / softcap).  slopes (H,) fp32: bias -slope * distance; or table (buckets,H) fp32
+    with buckets (2 reach + 1,) int32: learned bias by key - query distance (rel_buckets).  max_q / max_k: longest document, a sizing hint.
+    -> out (Tq,H,64) bf16, with train=True (out, state for packed_attn_bwd; table_grad=False: without the table's gradient).  Rows that no document covers: zero, or left alone in an `out` given by the
+    caller.  Offsets have to be non-decreasing.  NaN / inf outside a document never reaches it; inside, a NaN / inf key or value may reach any query of
+    its document.  Biases of -1e30 or less hide their keys."""
+    _chk(q, k, v, cu_q, cu_k, len_q, len_k, prefix, slopes, table, buckets, out)
+    q, k, v = _heads64(q, 'q'), _heads64(k, 'k'), _heads64(v, 'v')
+    dev = q.device
+    Tq, H, _ = q.shape
+    Tk, Hkv, _ = k.shape
+    if k.shape != v.shape or H < 1 or Hkv < 1 or H % Hkv or k.device != dev or v.device != dev:
+        raise E2KError(f'packed attention: k {tuple(k.shape)} and v {tuple(v.shape)} must match, on the device of q, with heads dividing {H}')
+    nd = _offsets(cu_q, 'cu_q', dev).numel() - 1
+    if cu_k is None:
+        if Tk != Tq:
+            raise E2KError('packed attention: cu_k is needed where k has other rows than q')
+        cu_k, len_k = cu_q, len_q if len_k is None else len_k
+        max_k = max_k or max_q
+    _offsets(cu_k, 'cu_k', dev, nd + 1)
+    for t, what in ((len_q, 'len_q'), (len_k, 'len_k'), (prefix, 'prefix')):
+        if t is not None:
+            _offsets(t, what, dev, nd)
+    if prefix is not None and not causal:
+        raise E2KError('packed attention: a prefix needs causal=True')
+    if max_q < 0 or max_k < 0:
+        raise E2KError('packed attention: max_q and max_k must not be negative')
+    scale, softcap, nb, reach = _score_args(H, dev, scale, softcap, slopes, table, buckets)
+    fill = out is None
+    if fill:
+        out = torch.empty((Tq, H, 64), dtype=bf16, device=dev)
+    elif out.shape != q.shape or out.dtype != bf16 or out.device != dev or out.stride(2) != 1 or out.stride(0) % 8 or out.stride(1) % 8 or out.data_ptr() % 16 \
+            or out.stride(0) >= 1 << 23 or not (out.stride(1) >= 64 and out.stride(0) >= H * 64 or (out.stride(0) >= 64 and out.stride(1) >= Tq * out.stride(0))):
+        raise E2KError('packed attention: out must be a (Tq, H, 64) bf16 tensor like q with 16-byte rows that do not overlap')
+    lo = lse2 = None
+    if train:
+        lo = torch.empty((Tq, H, 64), dtype=bf16, device=dev) if table is not None and table_grad else None
+        lse2 = torch.empty((H, Tq), dtype=f32, device=dev)
+    with _on_device(q):
+        _lib.get().e2k_packed_attn_fwd(_p(q), q.stride(0), q.stride(1), _p(k), k.stride(0), k.stride(1), _p(v), v.stride(0), v.stride(1), _p(cu_q), _p(cu_k),
+                                       _p(len_q), _p(len_k), _p(prefix), nd, Tq, Tk, H, Hkv, int(max_q), int(bool(causal)), scale, softcap, _p(slopes),
+                                       _p(table), _p(buckets), nb, reach, _p(out), out.stride(0), out.stride(1), _p(lo), _p(lse2), int(fill), _stream(q))
+    if not train:
+        return out
+    st = PackedAttnState()
+    st.q, st.k, st.v, st.cu_q, st.cu_k, st.len_q, st.len_k, st.prefix, st.max_q, st.max_k = q, k, v, cu_q, cu_k, len_q, len_k, prefix, int(max_q), int(max_k)
+    st.causal, st.scale, st.softcap, st.slopes, st.table, st.buckets, st.reach = bool(causal), scale, softcap, slopes, table, buckets, reach
+    st.out, st.lo, st.lse2 = out, lo, lse2
+    return out, st
+
+
+def packed_attn_bwd(st, dout, dtable=None):
+    """-> (dq, dk, dv, dtable): gradients of packed_attn_fwd(train=True), contiguous bf16 (rows that no document covers are zero); dtable fp32 (buckets,H) is
+    ADDED TO where given, fresh where not, None without a table or after a forward with table_grad=False"""
+    _chk(dout, dtable)
+    q, k, v = st.q, st.k, st.v
+    dout = _heads64(dout, 'dout')
+    dev = q.device
+    Tq, H, _ = q.shape
+    Tk, Hkv, _ = k.shape
+    if dout.shape != q.shape or dout.device != dev:
+        raise E2KError(f'packed attention: dout must match the output {tuple(q.shape)}, got {tuple(dout.shape)}')
+    nd = st.cu_q.numel() - 1
+    ws, acc = None, 0
+    if st.lo is None:
+        if dtable is not None:
+            raise E2KError('packed attention: dtable given, but the forward had no table or table_grad=False')
+    else:
+        if dtable is None:
+            dtable = torch.empty_like(st.table)
+        elif dtable.dtype != f32 or dtable.shape != st.table.shape or not dtable.is_contiguous() or dtable.device != dev:
+            raise E2KError('packed attention: dtable must be contiguous fp32 like the table')
+        else:
+            acc = 1
+        ws = torch.empty(_lib.get().e2k_query_packed_attn_bwd_ws_floats(nd, Tq, H, st.max_q, st.reach), dtype=f32, device=dev)
+    dq = torch.empty((Tq, H, 64), dtype=bf16, device=dev)
+    dk, dv = (torch.empty((Tk, Hkv, 64), dtype=bf16, device=dev) for _ in range(2))
+    delta = torch.empty((H, Tq), dtype=f32, device=dev)
+    out = st.out
+    with _on_device(q):
+        _lib.get().e2k_packed_attn_bwd(_p(dout), dout.stride(0), dout.stride(1), _p(q), q.stride(0), q.stride(1), _p(k), k.stride(0), k.stride(1), _p(v),
+                                       v.stride(0), v.stride(1), _p(st.cu_q), _p(st.cu_k), _p(st.len_q), _p(st.len_k), _p(st.prefix), nd, Tq, Tk, H, Hkv,
+                                       st.max_q, st.max_k, int(st.causal), st.scale, st.softcap, _p(st.slopes), _p(st.table), _p(st.buckets),
+                                       0 if st.table is None else st.table.shape[0], st.reach, _p(out), out.stride(0), out.stride(1), _p(st.lo), _p(st.lse2),
+                                       _p(delta), _p(dq), _p(dk), _p(dv), _p(dtable), acc, _p(ws), 1, _stream(q))
+    return dq, dk, dv, dtable
+
+
 # ------------------------------------------------------------------------------------------------ glue (csrc/glue.hip)
 
 def fill_(t, value=0):

@@ -346,6 +346,33 @@ int e2k_freq_attn_bwd(const void* dout, const void* qkv, int64_t ld, const void*
                       const float* sinb, float* dvfirst, int first_layer, void* dqkv, int64_t lddq, int B, int F, int N,
                       int H, void* stream);
 
+/* ---- attention over packed documents (beside e2k_attn_*: ragged utterances one behind the other instead of a padded batch) ----
+ * Q (Tq, H, 64), K / V (Tk, Hkv, 64) bf16, any token / head strides (s*, h*: elements, multiples of 8, token strides < 2^23); query head h reads key
+ * head h / (H / Hkv).  Document d's queries are the rows cu_q[d] .. cu_q[d + 1] - 1, its keys cu_k[d] .. cu_k[d + 1] - 1 (nd + 1 offsets on the
+ * device, never falling; offsets outside the tensors are cut off); len_q / len_k (device, may be NULL): only the first len rows of each slot
+ * count.  Query i of nq stands at position i + nk - nq.  It sees every key of its document (causal = 0), or the keys up to its position and the
+ * first prefix[d] keys (causal = 1; prefix device, may be NULL).
+ *   z = scale q.k;  c = softcap tanh(z / softcap) (softcap > 0, else z);  t = c - slopes[h] |j - i|  or  t = c + table[buckets[clamp(j - i) + reach]][h]
+ * (positions; slopes fp32 (H); table fp32 (nbuckets, H); buckets int32 (2 reach + 1) by key minus query distance, clamped at +-reach <= 512; one of
+ * slopes / table or neither), softmax over the visible keys, O = P V; a row that sees nothing is 0.  A bias of -1e30 or less hides its keys.
+ * O (Tq, H, 64) strided; rows that no document covers are zeroed with fill_gaps = 1, left alone with 0.  For the backward: lse2
+ * (H, Tq) fp32 (log2 domain), and with a table whose gradient is wanted Olo (Tq, H, 64) contiguous (what rounding to bf16 cut off O); NULL = not kept.
+ * max_q (max_k): the longest document, a sizing hint -- longer ones are computed all the same; 0 = unknown. */
+int e2k_packed_attn_fwd(const void* Q, int64_t sq, int64_t hq, const void* K, int64_t sk, int64_t hk, const void* V, int64_t sv, int64_t hv,
+                        const int32_t* cu_q, const int32_t* cu_k, const int32_t* len_q, const int32_t* len_k, const int32_t* prefix, int nd,
+                        int Tq, int Tk, int H, int Hkv, int max_q, int causal, float scale, float softcap, const float* slopes,
+                        const float* table, const int32_t* buckets, int nbuckets, int reach, void* O, int64_t so, int64_t ho, void* Olo,
+                        float* lse2, int fill_gaps, void* stream);
+/* dQ (Tq, H, 64), dK, dV (Tk, Hkv, 64) contiguous (uncovered rows as above); delta (H, Tq) scratch.  dtable (may be NULL): gradient of the table,
+ * (nbuckets, H) fp32, added to with accumulate = 1; Olo and ws (e2k_query_packed_attn_bwd_ws_floats floats) with dtable, else NULL.  Deterministic. */
+int64_t e2k_query_packed_attn_bwd_ws_floats(int nd, int Tq, int H, int max_q, int reach);
+int e2k_packed_attn_bwd(const void* dO, int64_t sg, int64_t hg, const void* Q, int64_t sq, int64_t hq, const void* K, int64_t sk, int64_t hk,
+                        const void* V, int64_t sv, int64_t hv, const int32_t* cu_q, const int32_t* cu_k, const int32_t* len_q,
+                        const int32_t* len_k, const int32_t* prefix, int nd, int Tq, int Tk, int H, int Hkv, int max_q, int max_k, int causal,
+                        float scale, float softcap, const float* slopes, const float* table, const int32_t* buckets, int nbuckets, int reach,
+                        const void* O, int64_t so, int64_t ho, const void* Olo, const float* lse2, float* delta, void* dQ, void* dK, void* dV,
+                        float* dtable, int accumulate, float* ws, int fill_gaps, void* stream);
+
 /* ---- MelSpec (e2_tts.py:248-290 -> torchaudio MelSpectrogram(n_fft=1024, hop, power=1, center, htk, norm=None)) ----
  * wave (B, nw) fp32 -> out (B, n_mels, 1 + nw/hop) fp32 = log(clamp(mel, 1e-5)).  window (n_fft) periodic Hann,
  * fb (n_fft/2+1, n_mels) filterbank, twc/tws (n_fft/2): cos/sin(2*pi*k/n_fft).  n_fft must be 1024.

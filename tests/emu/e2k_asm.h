@@ -32,6 +32,12 @@ inline s16x4_ lds_read_tr16_b64(const void* lds_ptr) {
 inline void lds_tr_issue(s16x4_& dst, const void* lds_ptr, int imm_off) { dst = lds_read_tr16_b64((const char*)lds_ptr + imm_off); }
 template <class... T> inline void lds_tr_wait(T&...) {}
 
+template <int STEP>
+inline void lds_tr_read8(s16x4_ (&d)[8], const void* lo0, const void* hi0, const void* lo1, const void* hi1) {
+    const void* a[4] = {lo0, hi0, lo1, hi1};
+    for (int i = 0; i < 8; ++i) d[i] = lds_read_tr16_b64((const char*)a[i & 3] + (i >> 2) * STEP);
+}
+
 inline float uniform_f(float v) { return v; }
 inline int uniform_i(int v) { return v; }
 inline float wave_sum_fast(float v) {          // same result up to summation order
