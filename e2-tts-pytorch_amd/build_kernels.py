@@ -23,7 +23,7 @@ FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-ffp-contract=f
 # Sources added since hipcc's packed-fp32 instructions were found to misbehave next to LDS-DMA traffic (tests/test_abi.py) are compiled without
 # them; the older ones keep the code they were measured and fenced with.
 NO_PACKED_FP32 = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
-NO_PACKED = {'layernorm.hip', 'packed_attn.hip'}
+NO_PACKED = {'attn_decode.hip', 'layernorm.hip', 'packed_attn.hip'}
 
 
 def _flags(src):

@@ -1,0 +1,281 @@
+// Attention of ONE query token per sequence over a long key / value cache (dim_head 64): the serving form of packed_attn.hip's scores.
+//
+//   q stands at position n - 1 of its sequence's n cached keys and sees all of them:  z = scale q.k, c = cap tanh(z / cap),
+//   t = c - slope_h |j - (n - 1)|  or  c + table[bucket(j - (n - 1)), h],  o = softmax(t) v;   n = 0: o = 0
+//
+// What bounds it: HBM, every K and V row of the cache once; the arithmetic has a factor of two to spare as long as it is not done by shuffles.
+// The G query heads of a key head are the columns of a 32 x 32 MFMA (unused columns cost nothing that matters), so a K / V row is read once for
+// all of them.  A wave walks its own share of the keys, 32 at a time, through an LDS ring of its own that LDS-DMA fills while the blocks before
+// are computed: no barriers, only counted waits.  The keys of a sequence are split evenly over `splits` workgroups of four waves by its actual
+// length; waves are joined in LDS, workgroups through a workspace by a second kernel (fixed order: the same bits every time).
+#include "e2k_device.h"
+#include "plan.h"
+#include <e2k_asm.h>
+#include "../../include/e2k.h"
+#include "attn_tile32.h"
+#include "attn_score.h"
+
+using namespace e2k;
+
+namespace {
+
+constexpr int NW = 4;                 // waves per workgroup
+constexpr int BLK = 8192;             // one ring stage: 32 keys of K and of V
+constexpr int STAGES = 2;
+constexpr int PART = 66;              // floats of a partial result: 64 columns, reference point, sum
+
+struct DecodeArgs {
+    const bf16_t *Q, *K, *V; long qb, qh, kb, kn, kh, vb, vn, vh, ob, oh;      // strides (elements): batch, key, head
+    const int* lens; int B, cap_n, H, Hkv, G, ngrp, splits;
+    float scale, cap;
+    const float *slopes, *table; const int* buckets; int nbuckets, R;
+    bf16_t* O; float* ws;
+};
+
+template <int BIAS, bool CAP>
+__global__ __launch_bounds__(NW * 64, 2) void attn_decode_kernel(DecodeArgs p) {
+    __shared__ __attribute__((aligned(16))) unsigned char smem[NW * STAGES * BLK];
+    __shared__ float ml[NW][2][32];
+    lds_declare(smem, sizeof(smem));
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform_i(tid >> 6);
+    const int l31 = lane & 31, hi = lane >> 5;
+    // key heads fastest: neighbouring workgroups read neighbouring parts of the same rows
+    int lin = (int)blockIdx.x;
+    const int hk = lin % p.Hkv; lin /= p.Hkv;
+    const int grp = lin % p.ngrp; lin /= p.ngrp;
+    const int split = lin % p.splits, b = lin / p.splits;
+    const int cols = min(32, p.G - 32 * grp), h0 = hk * p.G + 32 * grp;        // query heads h0 .. h0 + cols - 1
+    const int n = uniform_i(clampi(p.lens[b], 0, p.cap_n));
+    const int nblk = (n + 31) / 32;                                            // 32-key blocks of the sequence, shared evenly by splits x waves
+    const long parts = (long)p.splits * NW, me = (long)split * NW + wave;
+    const int b0 = (int)(nblk * me / parts), b1 = (int)(nblk * (me + 1) / parts);
+
+    const bool col = l31 < cols;
+    const int h = h0 + (col ? l31 : 0);
+    bf16x8 qf[4];
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks)
+        qf[ks] = col ? ld<bf16x8>(p.Q + (long)b * p.qb + (long)h * p.qh + ks * 16 + hi * 8) : bf16x8{0, 0, 0, 0, 0, 0, 0, 0};
+    const float sc2 = p.scale * LOG2E;
+    Cap cp{};
+    if (CAP) cp = cap_of(p.scale, p.cap);
+    const float sl2 = BIAS == 1 ? p.slopes[h] * LOG2E : 0.f;
+    const float far = BIAS == 2 ? p.table[(long)clampi(p.buckets[0], 0, p.nbuckets - 1) * p.H + h] * LOG2E : 0.f;
+
+    unsigned char* const ring = smem + wave * (STAGES * BLK);
+    const bf16_t* Kb = p.K + (long)b * p.kb + (long)hk * p.kh;
+    const bf16_t* Vb = p.V + (long)b * p.vb + (long)hk * p.vh;
+    const unsigned sk = (unsigned)(p.kn * 2), sv = (unsigned)(p.vn * 2);
+    auto issue = [&](int blk) __attribute__((always_inline)) {
+        unsigned char* S = ring + (blk - b0) % STAGES * BLK;
+        const char* ka = (const char*)(Kb + (long)blk * 32 * p.kn);
+        const char* va = (const char*)(Vb + (long)blk * 32 * p.vn);
+        const int last = n - 1 - blk * 32;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int r = u * 8 + (lane >> 3);
+            const unsigned row = (unsigned)min(swap23(r), last), c = (unsigned)(((lane & 7) ^ swz(r)) * 16);
+            glds16(ka + ((row & 0xffffffu) * (sk & 0xffffffu) + c), S + u * 1024);
+            glds16(va + ((row & 0xffffffu) * (sv & 0xffffffu) + c), S + 4096 + u * 1024);
+        }
+    };
+    int foff[4];
+    frag_offsets(l31, hi, foff);
+    const TrOff tro = tr_offsets(lane);
+    f32x16 o[2] = {zero16(), zero16()};
+    float m = M_INIT, l0 = 0.f, l1 = 0.f;
+    asm volatile("" ::"v"(qf[0]), "v"(qf[1]), "v"(qf[2]), "v"(qf[3]), "v"(sl2), "v"(far));
+#pragma unroll
+    for (int s = 0; s < STAGES; ++s)
+        if (b0 + s < b1) issue(b0 + s);
+    for (int blk = b0; blk < b1; ++blk) {
+        // blocks blk + 1 .. blk + STAGES - 1 stay in flight (eight copies each)
+        if (blk + STAGES - 1 < b1) wait_vmcnt<8 * (STAGES - 1)>();
+        else wait_vmcnt<0>();
+        wave_sync();
+        const unsigned char* Kt = ring + (blk - b0) % STAGES * BLK;
+        f32x16 s = zero16();
+        bf16x8 kf[4];
+        lds_read4(kf[0], kf[1], kf[2], kf[3], Kt + foff[0], Kt + foff[1], Kt + foff[2], Kt + foff[3]);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) s = mfma32(kf[ks], qf[ks], s);
+        if (CAP) cap16(s, cp);
+        const int kk = blk * 32, rel = kk + 8 * hi - (n - 1);
+        float t[16], c = 0.f;
+        const float f = CAP ? 1.f : sc2;
+        if (BIAS == 1) {
+            c = sl2 * (float)rel;                              // (every key lies at or before the query)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) t[r] = fmaf(s[r], f, sl2 * (float)reg_off(r));
+        } else if (BIAS == 2 && kk + 31 - (n - 1) > -p.R) {
+            cold_path();                                       // the last blocks only: within the table's reach
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int d = clampi(rel + reg_off(r), -p.R, 0) + p.R;
+                t[r] = fmaf(p.table[(long)clampi(p.buckets[d], 0, p.nbuckets - 1) * p.H + h], LOG2E, s[r] * f);
+            }
+        } else {
+            c = far;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) t[r] = s[r] * f;
+        }
+        if (kk + 32 > n) {
+            cold_path();
+            const int left = n - (kk + 8 * hi);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) t[r] = reg_off(r) < left ? t[r] : -__builtin_inff();
+        }
+        float mx = t[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, t[r]);
+        mx += c;
+        if (!wave_all(mx <= m + M_SLACK)) {
+            cold_path();
+            const float mn = fmaxf(m, fmaxf(mx, lane32_other(mx))), al = fast_exp2(m - mn);
+            l0 *= al;
+            l1 *= al;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) { o[0][r] *= al; o[1][r] *= al; }
+            m = mn;
+        }
+        const float mo = m - c;
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+            t[r] = fast_exp2(t[r] - mo);
+            t[r + 1] = fast_exp2(t[r + 1] - mo);
+            l0 += t[r];
+            l1 += t[r + 1];
+        }
+        const bf16x8 pf[2] = {pack8f(t), pack8f(t + 8)};
+        bf16x8 vf[2][2];
+        tr_frags(vf, Kt + 4096, tro);
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+            for (int db = 0; db < 2; ++db) o[db] = mfma32(vf[s2][db], pf[s2], o[db]);
+        wave_sync();                                           // every lane's reads of this stage are done (tr_frags waited): it may be refilled
+        if (blk + STAGES < b1) issue(blk + STAGES);
+    }
+    // join the waves: their accumulators through LDS (the rings are drained), reference points and sums beside them
+    float l = l0 + l1;
+    l += lane32_other(l);
+    __syncthreads();
+    float* acc = (float*)smem;                                 // [wave][column][64]
+    if (col) {
+#pragma unroll
+        for (int db = 0; db < 2; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[(wave * cols + l31) * DH + 32 * db + (r & 3) + 8 * (r >> 2) + 4 * hi] = o[db][r];
+        if (hi == 0) { ml[wave][0][l31] = m; ml[wave][1][l31] = l; }
+    }
+    __syncthreads();
+    for (int i = tid; i < cols * DH; i += NW * 64) {
+        const int cc = i / DH, d = i % DH;
+        float M = ml[0][0][cc], L = 0.f, a = 0.f;
+#pragma unroll
+        for (int w = 1; w < NW; ++w) M = fmaxf(M, ml[w][0][cc]);
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const float e = fast_exp2(ml[w][0][cc] - M);
+            L = fmaf(ml[w][1][cc], e, L);
+            a = fmaf(acc[(w * cols + cc) * DH + d], e, a);
+        }
+        if (p.splits == 1) {
+            p.O[(long)b * p.ob + (long)(h0 + cc) * p.oh + d] = f2bf(L == 0.f ? 0.f : a / L);
+        } else {
+            float* q = p.ws + (((long)b * p.H + h0 + cc) * p.splits + split) * PART;
+            q[d] = a;
+            if (d == 0) { q[DH] = M; q[DH + 1] = L; }
+        }
+    }
+}
+
+// one wave per (sequence, query head): lane = output column
+__global__ __launch_bounds__(256) void attn_decode_join_kernel(DecodeArgs p) {
+    const int lane = threadIdx.x & 63;
+    const long w = (long)blockIdx.x * 4 + uniform_i(threadIdx.x >> 6);
+    if (w >= (long)p.B * p.H) return;
+    const float* q = p.ws + w * p.splits * PART;
+    float M = M_INIT;
+    for (int s = lane; s < p.splits; s += 64) M = fmaxf(M, q[(long)s * PART + DH]);
+    M = wave_max(M);
+    float L = 0.f, a = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < p.splits; ++s) {
+        const float* r = q + (long)s * PART;
+        const float e = fast_exp2(r[DH] - M);
+        L = fmaf(r[DH + 1], e, L);
+        a = fmaf(r[lane], e, a);
+    }
+    p.O[(w / p.H) * p.ob + (w % p.H) * p.oh + lane] = f2bf(L == 0.f ? 0.f : a / L);
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+bool ok8(long s) { return s >= 0 && s % 8 == 0; }
+
+// Workgroups per (sequence, key head): about 1024 keys each (eight blocks a wave: the start of a wave is a few blocks' time), fewer keys where that
+// leaves the chip's 512 workgroup slots empty, never less than one block a wave; at most 128
+int splits_for(int B, int cap_n, int Hkv, int G) {
+    const long pairs = (long)B * Hkv * ((G + 31) / 32);
+    long s = (cap_n + 512) / 1024;
+    if (pairs * s < 512) s = (512 + pairs - 1) / pairs;
+    const long most = (cap_n + NW * 32 - 1) / (NW * 32);
+    if (s > most) s = most;
+    if (s > 128) s = 128;
+    return (int)(s < 1 ? 1 : s);
+}
+
+template <int BIAS, bool CAP> void run(const DecodeArgs& a, hipStream_t st) {
+    hipLaunchKernelGGL((attn_decode_kernel<BIAS, CAP>), dim3((unsigned)((long)a.B * a.splits * a.ngrp * a.Hkv)), dim3(NW * 64), 0, st, a);
+}
+
+int attn_decode_impl(const void* Q, int64_t qb, int64_t qh, const void* K, int64_t kb, int64_t kn, int64_t kh, const void* V, int64_t vb, int64_t vn,
+                     int64_t vh, const int32_t* lens, int B, int capacity, int H, int Hkv, float scale, float softcap, const float* slopes,
+                     const float* table, const int32_t* buckets, int nbuckets, int reach, void* O, int64_t ob, int64_t oh, float* ws, void* stream) {
+    if (B < 0 || capacity < 0 || H < 1 || Hkv < 1 || H % Hkv != 0) return E2K_ERR_SHAPE;
+    if (B == 0) return E2K_OK;
+    if (!Q || !O || !lens || (capacity > 0 && (!K || !V))) return E2K_ERR_ARG;
+    if (!(scale > 0.f) || !(scale < 1e30f) || !(softcap >= 0.f) || !(softcap < 1e30f) || (slopes && table)) return E2K_ERR_ARG;
+    if (table && (!buckets || nbuckets < 1 || reach < 0)) return E2K_ERR_SHAPE;
+    if (!aligned16(Q) || !aligned16(K) || !aligned16(V) || !ok8(qb) || !ok8(qh) || !ok8(kb) || !ok8(kn) || !ok8(kh) || !ok8(vb) || !ok8(vn) || !ok8(vh))
+        return E2K_ERR_ALIGN;
+    if (kn >= (1 << 23) || vn >= (1 << 23)) return E2K_ERR_SHAPE;
+    DecodeArgs a{};
+    a.Q = (const bf16_t*)Q; a.K = (const bf16_t*)K; a.V = (const bf16_t*)V;
+    a.qb = qb; a.qh = qh; a.kb = kb; a.kn = kn; a.kh = kh; a.vb = vb; a.vn = vn; a.vh = vh; a.ob = ob; a.oh = oh;
+    a.lens = lens; a.B = B; a.cap_n = capacity; a.H = H; a.Hkv = Hkv; a.G = H / Hkv; a.ngrp = (a.G + 31) / 32;
+    a.splits = splits_for(B, capacity, Hkv, a.G);
+    a.scale = scale; a.cap = softcap; a.slopes = slopes; a.table = table; a.buckets = buckets; a.nbuckets = nbuckets; a.R = reach;
+    a.O = (bf16_t*)O; a.ws = ws;
+    if (a.splits > 1 && !ws) return E2K_ERR_ARG;
+    if ((long)B * a.splits * a.ngrp * Hkv > 0x7fffffffL / (NW * 64)) return E2K_ERR_SHAPE;
+    hipStream_t st = (hipStream_t)stream;
+    const bool c = softcap > 0.f;
+    if (table) { if (c) run<2, true>(a, st); else run<2, false>(a, st); }
+    else if (slopes) { if (c) run<1, true>(a, st); else run<1, false>(a, st); }
+    else { if (c) run<0, true>(a, st); else run<0, false>(a, st); }
+    E2K_CHECK_LAUNCH();
+    if (a.splits > 1) {
+        hipLaunchKernelGGL(attn_decode_join_kernel, dim3((unsigned)(((long)B * H + 3) / 4)), dim3(256), 0, st, a);
+        E2K_CHECK_LAUNCH();
+    }
+    return E2K_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t e2k_query_attn_decode_ws_floats(int B, int capacity, int H, int Hkv) {
+    if (B < 1 || capacity < 0 || H < 1 || Hkv < 1 || H % Hkv != 0) return 0;
+    const int s = splits_for(B, capacity, Hkv, H / Hkv);
+    return s > 1 ? (int64_t)B * H * s * PART : 0;
+}
+int e2k_attn_decode(const void* Q, int64_t qb, int64_t qh, const void* K, int64_t kb, int64_t kn, int64_t kh, const void* V, int64_t vb, int64_t vn,
+                    int64_t vh, const int32_t* lens, int B, int capacity, int H, int Hkv, float scale, float softcap, const float* slopes,
+                    const float* table, const int32_t* buckets, int nbuckets, int reach, void* O, int64_t ob, int64_t oh, float* ws, void* stream) {
+    return e2k::dispatch("attn_decode", attn_decode_impl, Q, qb, qh, K, kb, kn, kh, V, vb, vn, vh, lens, B, capacity, H, Hkv, scale, softcap, slopes,
+                         table, buckets, nbuckets, reach, O, ob, oh, ws, stream);
+}
+
+}  // extern "C"

@@ -5,6 +5,7 @@
 namespace e2k {
 
 typedef short s16x4_ __attribute__((ext_vector_type(4)));
+typedef short bf16x8_ __attribute__((ext_vector_type(8)));
 
 // ds_read_b64_tr_b16: every lane passes the LDS address of 4 consecutive bf16 (8 B).  Within each
 // 16-lane group the 16x4 block {lane q -> its 4 elements} is transposed: lane q receives, as element j,
@@ -49,6 +50,17 @@ __device__ __forceinline__ void lds_tr_read8(s16x4_ (&d)[8], const void* lo0, co
         "s_waitcnt lgkmcnt(0)"
         : "=&v"(d[0]), "=&v"(d[1]), "=&v"(d[2]), "=&v"(d[3]), "=&v"(d[4]), "=&v"(d[5]), "=&v"(d[6]), "=&v"(d[7])
         : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "n"(STEP) : "memory");
+}
+
+// Four 16-byte LDS reads and their wait in one statement, for a kernel whose LDS-DMA copies into the next ring stage must stay in flight across
+// them (before its own ds_reads the compiler waits for every copy when it cannot tell the stages apart).
+__device__ __forceinline__ void lds_read4(bf16x8_& r0, bf16x8_& r1, bf16x8_& r2, bf16x8_& r3, const void* p0, const void* p1, const void* p2, const void* p3) {
+    typedef const __attribute__((address_space(3))) void* lp_t;
+    const unsigned a0 = (unsigned)(unsigned long long)(lp_t)(p0), a1 = (unsigned)(unsigned long long)(lp_t)(p1);
+    const unsigned a2 = (unsigned)(unsigned long long)(lp_t)(p2), a3 = (unsigned)(unsigned long long)(lp_t)(p3);
+    asm volatile(
+        "ds_read_b128 %0, %4\n ds_read_b128 %1, %5\n ds_read_b128 %2, %6\n ds_read_b128 %3, %7\n s_waitcnt lgkmcnt(0)"
+        : "=&v"(r0), "=&v"(r1), "=&v"(r2), "=&v"(r3) : "v"(a0), "v"(a1), "v"(a2), "v"(a3) : "memory");
 }
 
 // raw v_exp_f32 (2^x, no denormal fix-up: results below 2^-126 flush to 0) and v_rcp_f32 (1 ulp)
@@ -152,7 +164,6 @@ __device__ __forceinline__ unsigned long long sload64(const unsigned long long* 
 // v_mfma_f32_32x32x16_bf16: A 32x16 (lane l: row l & 31, k-slots 8 (l >> 5) .. + 7), B 16x32 (lane l: column l & 31, the same
 // k-slots), C / D 32x32: lane l holds column l & 31, register r <-> row (r & 3) + 8 (r >> 2) + 4 (l >> 5)
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef short bf16x8_ __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ f32x16 mfma32(bf16x8_ a, bf16x8_ b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 // v_permlane32_swap_b32: lanes 32..63 of `a` trade places with lanes 0..31 of `b` (the other two halves stay)
 __device__ __forceinline__ void lane32_swap(unsigned& a, unsigned& b) {

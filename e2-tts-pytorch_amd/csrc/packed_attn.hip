@@ -31,18 +31,14 @@
 #include <e2k_asm.h>
 #include "../../include/e2k.h"
 #include "attn_tile32.h"
+#include "attn_score.h"
 
 using namespace e2k;
 
 namespace {
 
-constexpr int DH = 64;
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr float LN2 = 0.6931471805599453f;
 constexpr int STAGE = 16384;          // one ring stage: two [64][64] bf16 tiles
-constexpr float M_INIT = -1e30f;      // running maximum before any visible key
 constexpr float LSE_EMPTY = 1e30f;    // log-sum-exp of a row that sees nothing: exp2(t - it) is 0
-constexpr float M_SLACK = 8.f;        // (log2) how far a score may exceed the reference point before the accumulators are rescaled
 constexpr int PADL = 64;              // entries of the distance table beyond its reach on either side (a block's distances spread over 63)
 constexpr int REACH_MAX = 512;
 constexpr int GAP_PARTS = 8;          // workgroups per gap between documents
@@ -62,7 +58,6 @@ struct PAArgs {
     int nt, nwork;                                     // row tiles per (document, head) of this grid; workgroups that compute
 };
 
-__device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
 // rows of document d, kept inside [0, total) whatever the offsets say
 struct Span { int at, n; };
 __device__ __forceinline__ Span span(const int* cu, const int* len, int d, int total) {
@@ -122,26 +117,6 @@ __device__ __forceinline__ void fill_gap(const int* cu, const int* len, int nd, 
 
 // ------------------------------------------------------------------------------------------------ scores
 
-__device__ __forceinline__ constexpr int reg_off(int r) { return 16 * (r >> 3) + (r & 7); }      // row of accumulator r within its block (+ 8 hi)
-
-// tanh cap:  out tanh(s kx)  with out = cap log2(e).  |s kx| <= 0.3 (a wave vote): minimax of tanh(x) / x in x^2, four terms, relative error
-// 1e-8 (below fp32's half step); beyond: 1 - 2 / (2^(2 x log2 e) + 1)
-constexpr float CAP_POLY_MAX = 0.3f;
-struct Cap { float a0, a1, a2, a3, k2, out, lim; };
-__device__ __forceinline__ Cap cap_of(float scale, float cap) {
-    Cap c;
-    const float kx = scale / cap, k2 = kx * kx;
-    c.out = cap * LOG2E;
-    const float k1 = c.out * kx;
-    c.a0 = k1;
-    c.a1 = k1 * k2 * -0.33332962f;
-    c.a2 = k1 * k2 * k2 * 0.13312598f;
-    c.a3 = k1 * k2 * k2 * k2 * -0.050222438f;
-    c.k2 = 2.f * LOG2E * kx;
-    c.lim = CAP_POLY_MAX / kx;
-    return c;
-}
-
 // One block of 32 rows x 32 columns of scores, 16 of them in a lane: distance (key - query position) of register r is  rel + SGN reg_off(r).
 //   z[r]: capped score, t[r]: z plus the part of the bias that differs between registers, c: the part that does not (per lane); log2 domain.
 //   lo: smallest distance of the block's first row to its columns, so that the block spans distances lo - 31 .. lo + 31
@@ -159,21 +134,7 @@ template <int BIAS, bool CAP, int SGN> struct Scorer {
         }
     }
     __device__ __forceinline__ void block(f32x16& z, float (&t)[16], float& c, int rel, int lo) const {
-        if (CAP) {
-            float a = 0.f;
-#pragma unroll
-            for (int r = 0; r < 16; r += 2) a = fmaxf(fmaxf(fabsf(z[r]), fabsf(z[r + 1])), a);
-            if (wave_all(a <= cp.lim)) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const float w = z[r] * z[r];
-                    z[r] *= fmaf(fmaf(fmaf(w, cp.a3, cp.a2), w, cp.a1), w, cp.a0);
-                }
-            } else {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) z[r] = fmaf(-2.f * cp.out, fast_rcp(fast_exp2(z[r] * cp.k2) + 1.f), cp.out);
-            }
-        }
+        if (CAP) cap16(z, cp);
         c = 0.f;
         const float f = CAP ? 1.f : sc2;
         if (BIAS == 0) {
@@ -242,21 +203,6 @@ struct Stager {
         }
     }
 };
-
-// transposed fragments of a block (32 tile rows at T): f[s2][db] = columns 32 db + l31, rows 16 s2 + 8 hi .. + 7
-__device__ __forceinline__ void tr_frags(bf16x8 (&f)[2][2], const unsigned char* T, const TrOff& t) {
-    s16x4_ d[8];
-    lds_tr_read8<2048>(d, T + t.lo[0], T + t.hi_[0], T + t.lo[1], T + t.hi_[1]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i >> 1][i & 1] = __builtin_shufflevector(d[2 * i], d[2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
-}
-
-__device__ __forceinline__ f32x16 zero16() {
-    f32x16 z;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) z[r] = 0.f;
-    return z;
-}
 
 // ------------------------------------------------------------------------------------------------ forward
 

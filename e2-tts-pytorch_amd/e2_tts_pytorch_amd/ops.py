@@ -1196,6 +1196,40 @@ def packed_attn_bwd(st, dout, dtable=None):
     return dq, dk, dv, dtable
 
 
+def attn_decode(q, k_cache, v_cache, lens, *, scale=None, softcap=0., slopes=None, table=None, buckets=None, out=None):
+    """One query token per sequence over its cached keys: q (B,H,64), k_cache / v_cache (B,capacity,Hkv,64) bf16 (any strides with 16-byte rows: head-major
+    caches as transposed views, slices of larger ones), lens (B,) int32 on the device: sequence b has lens[b] keys (cut off at the capacity), the query
+    is the last of them.  Scores as in packed_attn_fwd with causal=True.  -> out (B,H,64) bf16; zero where lens is 0.  Cache rows past lens are not read"""
+    _chk(q, k_cache, v_cache, lens, slopes, table, buckets, out)
+    if q.dim() != 3 or q.shape[2] != 64 or q.dtype != bf16:
+        raise E2KError(f'attn_decode: q must be (sequences, heads, 64) bf16, got {q.dtype} {tuple(q.shape)}')
+    B, H, _ = q.shape
+    dev = q.device
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[0] != B or k_cache.shape[3] != 64 or k_cache.dtype != bf16 or v_cache.dtype != bf16 \
+            or H < 1 or k_cache.shape[2] < 1 or H % k_cache.shape[2] or k_cache.device != dev or v_cache.device != dev:
+        raise E2KError(f'attn_decode: caches must be ({B}, capacity, heads dividing {H}, 64) bf16 on the device of q, got {tuple(k_cache.shape)}, {tuple(v_cache.shape)}')
+    cap, Hkv = k_cache.shape[1:3]
+    sk, sv = k_cache.stride(), v_cache.stride()
+    if sk[3] != 1 or sv[3] != 1 or any(x % 8 for x in sk[:3] + sv[:3]) or sk[1] >= 1 << 23 or sv[1] >= 1 << 23 or k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16:
+        raise E2KError('attn_decode: cache rows must be contiguous and 16-byte aligned, less than 2^23 elements apart (a cache is not copied)')
+    if lens.dtype != torch.int32 or lens.shape != (B,) or not lens.is_contiguous() or lens.device != dev:
+        raise E2KError(f'attn_decode: lens must be contiguous int32 ({B},) on the device of q')
+    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+        q = q.contiguous()
+    scale, softcap, nb, reach = _score_args(H, dev, scale, softcap, slopes, table, buckets, 'attn_decode')
+    if out is None:
+        out = torch.empty((B, H, 64), dtype=bf16, device=dev)
+    elif out.shape != (B, H, 64) or out.dtype != bf16 or out.stride(2) != 1 or out.device != dev or (B > 1 and out.stride(0) < 64) or (H > 1 and out.stride(1) < 64):
+        raise E2KError('attn_decode: out must be (sequences, heads, 64) bf16 like q, with contiguous rows that do not overlap')
+    L = _lib.get()
+    n = L.e2k_query_attn_decode_ws_floats(B, cap, H, Hkv)
+    ws = torch.empty(n, dtype=f32, device=dev) if n else None
+    with _on_device(q):
+        L.e2k_attn_decode(_p(q), q.stride(0), q.stride(1), _p(k_cache), sk[0], sk[1], sk[2], _p(v_cache), sv[0], sv[1], sv[2], _p(lens), B, cap, H, Hkv, scale,
+                          softcap, _p(slopes), _p(table), _p(buckets), nb, reach, _p(out), out.stride(0), out.stride(1), _p(ws), _stream(q))
+    return out
+
+
 # ------------------------------------------------------------------------------------------------ glue (csrc/glue.hip)
 
 def fill_(t, value=0):

@@ -373,6 +373,16 @@ int e2k_packed_attn_bwd(const void* dO, int64_t sg, int64_t hg, const void* Q, i
                         const void* O, int64_t so, int64_t ho, const void* Olo, const float* lse2, float* delta, void* dQ, void* dK, void* dV,
                         float* dtable, int accumulate, float* ws, int fill_gaps, void* stream);
 
+/* One query token per sequence over a cache (the same scores): Q / O (B, H, 64), K / V (B, capacity, Hkv, 64) bf16 with any batch / key / head
+ * strides (elements, multiples of 8, key strides < 2^23; O's any); sequence b has lens[b] keys (device, cut off at 0 and capacity), its query stands
+ * on the last of them and sees them all; no keys: O = 0.  Keys past lens[b] are not read.  buckets: distances 0 and below of the map are used.
+ * ws: e2k_query_attn_decode_ws_floats floats (0: NULL will do). */
+int64_t e2k_query_attn_decode_ws_floats(int B, int capacity, int H, int Hkv);
+int e2k_attn_decode(const void* Q, int64_t qb, int64_t qh, const void* K, int64_t kb, int64_t kn, int64_t kh, const void* V, int64_t vb,
+                    int64_t vn, int64_t vh, const int32_t* lens, int B, int capacity, int H, int Hkv, float scale, float softcap,
+                    const float* slopes, const float* table, const int32_t* buckets, int nbuckets, int reach, void* O, int64_t ob, int64_t oh,
+                    float* ws, void* stream);
+
 /* ---- MelSpec (e2_tts.py:248-290 -> torchaudio MelSpectrogram(n_fft=1024, hop, power=1, center, htk, norm=None)) ----
  * wave (B, nw) fp32 -> out (B, n_mels, 1 + nw/hop) fp32 = log(clamp(mel, 1e-5)).  window (n_fft) periodic Hann,
  * fb (n_fft/2+1, n_mels) filterbank, twc/tws (n_fft/2): cos/sin(2*pi*k/n_fft).  n_fft must be 1024.

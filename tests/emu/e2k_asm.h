@@ -75,6 +75,9 @@ inline float fast_rcp(float x) { return 1.0f / x; }
 // host model of v_mfma_f32_32x32x16_bf16 (fragment layout: csrc/e2k_asm.h)
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short bf16x8_ __attribute__((ext_vector_type(8)));
+inline void lds_read4(bf16x8_& r0, bf16x8_& r1, bf16x8_& r2, bf16x8_& r3, const void* p0, const void* p1, const void* p2, const void* p3) {
+    memcpy(&r0, p0, 16); memcpy(&r1, p1, 16); memcpy(&r2, p2, 16); memcpy(&r3, p3, 16);
+}
 inline f32x16 mfma32(bf16x8_ a, bf16x8_ b, f32x16 c) {
     struct AB { bf16x8_ a, b; };
     emu::Wave& w = emu::cur_wave();

@@ -386,3 +386,107 @@ def test_packed_attention_large(c):
     install(None, False)
     _lib.get()
     check(Case(**c), 'cuda')
+
+
+# ------------------------------------------------------------------------------------------------ one query token per sequence
+
+def decode_case(lens, cap_n, H=4, Hkv=None, cap=0., bias='none', buckets=8, reach=24, seed=0, gain=1.5):
+    """-> (q, k, v, lens, keyword arguments), exact output and its error bound: each sequence is a one-query document over its cached keys"""
+    Hkv = Hkv or H
+    B = len(lens)
+    c = Case([1] * B, kl=[cap_n] * B, H=H, Hkv=Hkv, mask='causal', cap=cap, bias=bias, buckets=buckets, reach=reach, seed=seed, gain=gain,
+             nk=[min(max(n, 0), cap_n) for n in lens])
+    want, bound = c.exact()
+    # two further roundings-free joins (waves, workgroups) of fp32 partial sums: 2 x 128 additions at most, far below the probabilities' bf16 rounding
+    return c, want['out'], bound['out'] * (1 + 256 * U / HALF)
+
+
+def decode(c, lens, cap_n, dev, **more):
+    from e2_tts_pytorch_amd import ops
+    to = lambda t: None if t is None else t.to(dev)  # noqa: E731
+    B = len(lens)
+    k, v = (t.view(B, cap_n, c.Hkv, 64).clone() for t in (c.k, c.v))
+    for b, n in enumerate(lens):                 # what lies behind a sequence's keys is never read
+        k[b, max(n, 0):], v[b, max(n, 0):] = float('nan'), float('inf')
+    kw = dict(softcap=c.cap, slopes=to(c.slopes), table=to(c.table), buckets=to(c.map))
+    kw.update(more)
+    return ops.attn_decode(c.q.to(dev), k.to(dev), v.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev), **kw)
+
+
+@pytest.mark.parametrize('bias', BIASES)
+@pytest.mark.parametrize('cap', [0., 20.])
+def test_attn_decode(dev, landing, bias, cap):
+    lens, cap_n = [1, 33, 0, 200, 150, 64], 200
+    c, want, bound = decode_case(lens, cap_n, cap=cap, bias=bias)
+    held(decode(c, lens, cap_n, dev), want, bound, 'out')
+
+
+def test_attn_decode_grouped_heads(dev):
+    for H, Hkv in ((4, 2), (3, 1), (40, 1)):                     # (more query heads than an MFMA has columns: two passes over the keys)
+        c, want, bound = decode_case([70, 40], 80, H=H, Hkv=Hkv, bias='alibi')
+        held(decode(c, [70, 40], 80, dev), want, bound, 'out')
+
+
+def test_attn_decode_cut_lengths(dev):
+    """lengths outside 0 .. capacity are cut off"""
+    c, want, bound = decode_case([-3, 10 ** 6], 50)
+    held(decode(c, [-3, 10 ** 6], 50, dev), want, bound, 'out')
+
+
+def test_attn_decode_strides(dev):
+    """a head-major cache, a slice of a longer one, strided q and out"""
+    from e2_tts_pytorch_amd import ops
+    lens, n = [50, 61], 64
+    c, want, bound = decode_case(lens, n, H=2)
+    B = 2
+    k, v = (t.view(B, n, 2, 64) for t in (c.k, c.v))
+    kh = k.transpose(1, 2).contiguous().to(dev).transpose(1, 2)
+    vl = torch.full((B, 3 * n, 2, 64), float('nan'), dtype=bf16, device=dev)
+    vl[:, n:2 * n] = v.to(dev)
+    L = torch.tensor(lens, dtype=torch.int32, device=dev)
+    buf = torch.full((B, 3, 64), 7., dtype=bf16, device=dev)
+    qs = torch.zeros(B, 2, 3, 64, dtype=bf16, device=dev)[:, :, 1]
+    qs.copy_(c.q)
+    out = ops.attn_decode(qs, kh, vl[:, n:2 * n], L, out=buf[:, 1:])
+    held(out, want, bound, 'out')
+    assert (buf[:, 0] == 7.).all()
+
+
+def test_attn_decode_matches_packed(dev):
+    """the same scores as a packed call with one query per document"""
+    from e2_tts_pytorch_amd import ops
+    lens, n = [90, 13], 96
+    c, want, bound = decode_case(lens, n, bias='table', cap=25.)
+    a, kw = c.args(dev)
+    held(ops.packed_attn_fwd(*a, **kw), want, bound, 'packed')
+    held(decode(c, lens, n, dev), want, bound, 'decode')
+
+
+def test_attn_decode_refusals(emu):
+    from e2_tts_pytorch_amd import ops
+    q, k, L = torch.zeros(2, 4, 64, dtype=bf16), torch.zeros(2, 8, 2, 64, dtype=bf16), torch.ones(2, dtype=torch.int32)
+    f = ops.attn_decode
+    assert f(q, k, k, L).shape == (2, 4, 64)
+    assert f(q[:0], k[:0], k[:0], L[:0]).shape == (0, 4, 64)
+    bad = [lambda: f(q.float(), k, k, L), lambda: f(q, k[:1], k[:1], L), lambda: f(q, k, k[:, :4], L), lambda: f(q, k[..., :32], k[..., :32], L),
+           lambda: f(q[:, :3], k, k, L), lambda: f(q, k, k, L.long()), lambda: f(q, k, k, L[:1]), lambda: f(q, k.transpose(2, 3), k.transpose(2, 3), L),
+           lambda: f(q, torch.zeros(2 * 8 * 2 * 64 + 1, dtype=bf16)[1:].view(2, 8, 2, 64), k, L), lambda: f(q, k, k, L, softcap=-1.),
+           lambda: f(q, k, k, L, slopes=torch.ones(2)), lambda: f(q, k, k, L, out=torch.zeros(2, 4, 64)), lambda: f(q, k.float(), k.float(), L)]
+    for i, g in enumerate(bad):
+        with pytest.raises(ops.E2KError):
+            g()
+            print('not refused:', i)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('lens,n,kw', [([4128, 2000, 1, 3333], 4128, dict(H=16, bias='table', buckets=32, reach=128)),
+                                       ([30000, 17], 30011, dict(H=8, Hkv=2, bias='alibi', cap=50.)), ([640], 640, dict(H=16))], ids=['batch', 'long', 'one'])
+def test_attn_decode_large(lens, n, kw):
+    from e2_tts_pytorch_amd import _lib
+    from emu.install import install
+    install(None, False)
+    _lib.get()
+    c, want, bound = decode_case(lens, n, **kw)
+    out = decode(c, lens, n, 'cuda')
+    held(out, want, bound, 'out')
+    assert torch.equal(out, decode(c, lens, n, 'cuda'))
