@@ -7,8 +7,10 @@ import types as _types
 
 from .backbone import Transformer
 from .e2_tts import E2TTS, DurationPredictor, MelSpec, E2TTSReturn, LossBreakdown
+from .packed import LayerNorm, RelativePositionBias, attn_decode, layer_norm, packed_attention
 
-__all__ = ['Transformer', 'E2TTS', 'DurationPredictor', 'MelSpec', 'E2TTSReturn', 'LossBreakdown', 'install_as_reference', 'set_runtime_env']
+__all__ = ['Transformer', 'E2TTS', 'DurationPredictor', 'MelSpec', 'E2TTSReturn', 'LossBreakdown', 'LayerNorm', 'RelativePositionBias', 'attn_decode',
+           'layer_norm', 'packed_attention', 'install_as_reference', 'set_runtime_env']
 
 
 def install_as_reference():
