@@ -81,19 +81,20 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_decode_kernel(DecodeArgs p) {
     };
     int foff[4];
     frag_offsets(l31, hi, foff);
-    const TrOff tro = tr_offsets(lane);
+    const TrAddr tra = tr_addr(ring, lane);
     f32x16 o[2] = {zero16(), zero16()};
     float m = M_INIT, l0 = 0.f, l1 = 0.f;
     asm volatile("" ::"v"(qf[0]), "v"(qf[1]), "v"(qf[2]), "v"(qf[3]), "v"(sl2), "v"(far));
 #pragma unroll
     for (int s = 0; s < STAGES; ++s)
         if (b0 + s < b1) issue(b0 + s);
-    for (int blk = b0; blk < b1; ++blk) {
+    auto step = [&](auto stage_, int blk) __attribute__((always_inline)) {
+        constexpr int S = decltype(stage_)::value * BLK;
         // blocks blk + 1 .. blk + STAGES - 1 stay in flight (eight copies each)
         if (blk + STAGES - 1 < b1) wait_vmcnt<8 * (STAGES - 1)>();
         else wait_vmcnt<0>();
         wave_sync();
-        const unsigned char* Kt = ring + (blk - b0) % STAGES * BLK;
+        const unsigned char* Kt = ring + S;
         f32x16 s = zero16();
         bf16x8 kf[4];
         lds_read4(kf[0], kf[1], kf[2], kf[3], Kt + foff[0], Kt + foff[1], Kt + foff[2], Kt + foff[3]);
@@ -125,36 +126,53 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_decode_kernel(DecodeArgs p) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) t[r] = reg_off(r) < left ? t[r] : -__builtin_inff();
         }
-        float mx = t[0];
+        // probabilities against the reference point m; a sum past 2^60 (the first block's overflows) takes the block's maximum and starts over
+        bf16x8 pf[2];
+        float la, lb;
+        auto probs = [&]() __attribute__((always_inline)) {
+            const float mo = m - c;
+            float e[16];
 #pragma unroll
-        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, t[r]);
-        mx += c;
-        if (!wave_all(mx <= m + M_SLACK)) {
+            for (int r = 0; r < 16; ++r) e[r] = fast_exp2(t[r] - mo);
+            pf[0] = pack8f(e);
+            pf[1] = pack8f(e + 8);
+            la = l0;
+            lb = l1;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                la = add_bf16_pair(__builtin_bit_cast(u32x4, pf[0])[i], la);
+                lb = add_bf16_pair(__builtin_bit_cast(u32x4, pf[1])[i], lb);
+            }
+        };
+        probs();
+        if (!wave_all(la + lb < L_MAX)) {
             cold_path();
+            float mx = t[0];
+#pragma unroll
+            for (int r = 1; r < 16; ++r) mx = fmaxf(mx, t[r]);
+            mx += c;
             const float mn = fmaxf(m, fmaxf(mx, lane32_other(mx))), al = fast_exp2(m - mn);
             l0 *= al;
             l1 *= al;
 #pragma unroll
             for (int r = 0; r < 16; ++r) { o[0][r] *= al; o[1][r] *= al; }
             m = mn;
+            probs();
         }
-        const float mo = m - c;
-#pragma unroll
-        for (int r = 0; r < 16; r += 2) {
-            t[r] = fast_exp2(t[r] - mo);
-            t[r + 1] = fast_exp2(t[r + 1] - mo);
-            l0 += t[r];
-            l1 += t[r + 1];
-        }
-        const bf16x8 pf[2] = {pack8f(t), pack8f(t + 8)};
+        l0 = la;
+        l1 = lb;
         bf16x8 vf[2][2];
-        tr_frags(vf, Kt + 4096, tro);
+        tr_frags<S + 4096>(vf, tra);
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
             for (int db = 0; db < 2; ++db) o[db] = mfma32(vf[s2][db], pf[s2], o[db]);
         wave_sync();                                           // every lane's reads of this stage are done (tr_frags waited): it may be refilled
         if (blk + STAGES < b1) issue(blk + STAGES);
+    };
+    for (int blk = b0; blk < b1; blk += 2) {
+        step(Int<0>{}, blk);
+        if (blk + 1 < b1) step(Int<1>{}, blk + 1);
     }
     // join the waves: their accumulators through LDS (the rings are drained), reference points and sums beside them
     float l = l0 + l1;

@@ -10,13 +10,14 @@ using namespace e2k;
 constexpr int DH = 64;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float M_INIT = -1e30f;      // running maximum before any visible key
-constexpr float M_SLACK = 8.f;        // (log2) how far a score may exceed the reference point before the accumulators are rescaled
+constexpr float L_MAX = 0x1p60f;      // largest sum of a row (per half-wave) before the accumulators are rescaled
 
+template <int N> struct Int { static constexpr int value = N; };
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
 __device__ __forceinline__ constexpr int reg_off(int r) { return 16 * (r >> 3) + (r & 7); }      // row of accumulator r within its block (+ 8 hi)
 
 // tanh cap:  out tanh(s kx)  with out = cap log2(e).  |s kx| <= 0.3 (a wave vote): minimax of tanh(x) / x in x^2, four terms, relative error
-// 1e-8 (below fp32's half step); beyond: 1 - 2 / (2^(2 x log2 e) + 1)
+// 1e-8 (below fp32's half step); beyond: 1 - 2 / (2^(2 x log2 e) + 1), absolute error 2^-22
 constexpr float CAP_POLY_MAX = 0.3f;
 struct Cap { float a0, a1, a2, a3, k2, out, lim; };
 __device__ __forceinline__ Cap cap_of(float scale, float cap) {
@@ -43,15 +44,22 @@ __device__ __forceinline__ void cap16(f32x16& z, const Cap& cp) {
             z[r] *= fmaf(fmaf(fmaf(w, cp.a3, cp.a2), w, cp.a1), w, cp.a0);
         }
     } else {
+        cold_path();
 #pragma unroll
         for (int r = 0; r < 16; ++r) z[r] = fmaf(-2.f * cp.out, fast_rcp(fast_exp2(z[r] * cp.k2) + 1.f), cp.out);
     }
 }
 
-// transposed fragments of a block (32 tile rows at T): f[s2][db] = columns 32 db + l31, rows 16 s2 + 8 hi .. + 7
-__device__ __forceinline__ void tr_frags(bf16x8 (&f)[2][2], const unsigned char* T, const TrOff& t) {
+// transposed fragments of a block of 32 tile rows OFF bytes behind the tile image that the addresses were made for:
+// f[s2][db] = columns 32 db + l31, rows 16 s2 + 8 hi .. + 7
+struct TrAddr { unsigned lo[2], hi_[2]; };
+__device__ __forceinline__ TrAddr tr_addr(const unsigned char* tile, int lane) {
+    const TrOff t = tr_offsets(lane);
+    return TrAddr{{lds_addr(tile + t.lo[0]), lds_addr(tile + t.lo[1])}, {lds_addr(tile + t.hi_[0]), lds_addr(tile + t.hi_[1])}};
+}
+template <int OFF> __device__ __forceinline__ void tr_frags(bf16x8 (&f)[2][2], const TrAddr& t) {
     s16x4_ d[8];
-    lds_tr_read8<2048>(d, T + t.lo[0], T + t.hi_[0], T + t.lo[1], T + t.hi_[1]);
+    lds_tr_read8<OFF, 2048>(d, t.lo[0], t.hi_[0], t.lo[1], t.hi_[1]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i >> 1][i & 1] = __builtin_shufflevector(d[2 * i], d[2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
 }

@@ -38,18 +38,24 @@ template <class... T> __device__ __forceinline__ void lds_tr_wait(T&... r) {
 // Eight transposing reads and their wait in ONE statement: lo / hi of column block 0, lo / hi of column block 1 at the byte addresses given,
 // then the same `step` bytes further on.  Nothing of the compiler's can come between a read in flight and its destination registers, and
 // LDS-DMA copies in flight are not waited for (which the builtin's ordering would do).  The caller's LDS image must be complete.
-template <int STEP>
-__device__ __forceinline__ void lds_tr_read8(s16x4_ (&d)[8], const void* lo0, const void* hi0, const void* lo1, const void* hi1) {
-    typedef const __attribute__((address_space(3))) void* lp_t;
-    const unsigned a0 = (unsigned)(unsigned long long)(lp_t)(lo0), a1 = (unsigned)(unsigned long long)(lp_t)(hi0);
-    const unsigned a2 = (unsigned)(unsigned long long)(lp_t)(lo1), a3 = (unsigned)(unsigned long long)(lp_t)(hi1);
+// (OFF, STEP: compile-time byte offsets)
+__device__ __forceinline__ unsigned lds_addr(const void* p) { return (unsigned)(unsigned long long)(const __attribute__((address_space(3))) void*)(p); }
+template <int OFF, int STEP>
+__device__ __forceinline__ void lds_tr_read8(s16x4_ (&d)[8], unsigned lo0, unsigned hi0, unsigned lo1, unsigned hi1) {
     asm volatile(
-        "ds_read_b64_tr_b16 %0, %8\n ds_read_b64_tr_b16 %1, %9\n ds_read_b64_tr_b16 %2, %10\n ds_read_b64_tr_b16 %3, %11\n"
-        "ds_read_b64_tr_b16 %4, %8 offset:%12\n ds_read_b64_tr_b16 %5, %9 offset:%12\n"
-        "ds_read_b64_tr_b16 %6, %10 offset:%12\n ds_read_b64_tr_b16 %7, %11 offset:%12\n"
+        "ds_read_b64_tr_b16 %0, %8 offset:%12\n ds_read_b64_tr_b16 %1, %9 offset:%12\n"
+        "ds_read_b64_tr_b16 %2, %10 offset:%12\n ds_read_b64_tr_b16 %3, %11 offset:%12\n"
+        "ds_read_b64_tr_b16 %4, %8 offset:%13\n ds_read_b64_tr_b16 %5, %9 offset:%13\n"
+        "ds_read_b64_tr_b16 %6, %10 offset:%13\n ds_read_b64_tr_b16 %7, %11 offset:%13\n"
         "s_waitcnt lgkmcnt(0)"
         : "=&v"(d[0]), "=&v"(d[1]), "=&v"(d[2]), "=&v"(d[3]), "=&v"(d[4]), "=&v"(d[5]), "=&v"(d[6]), "=&v"(d[7])
-        : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "n"(STEP) : "memory");
+        : "v"(lo0), "v"(hi0), "v"(lo1), "v"(hi1), "n"(OFF), "n"(OFF + STEP) : "memory");
+}
+
+// acc + lo + hi of a packed bf16 pair (v_dot2c_f32_bf16 with ones)
+__device__ __forceinline__ float add_bf16_pair(unsigned pair, float acc) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, pair), __builtin_bit_cast(b2, 0x3f803f80u), acc, false);
 }
 
 // Four 16-byte LDS reads and their wait in one statement, for a kernel whose LDS-DMA copies into the next ring stage must stay in flight across

@@ -18,8 +18,9 @@
 // and sixteen wave-uniform addends (the addend of the multiply-add that scales the score anyway); where a block lies beyond the table's reach
 // the learned bias is one constant.  Only blocks that cross the diagonal (or lie within reach) take |distance| (an LDS lookup) per score.
 //
-// Softmax: running maximum with a lazy rescale -- the accumulators are rescaled only when a block's maximum exceeds the reference point by 2^8
-// (fp32 sums and bf16 probabilities lose nothing by a common factor), which in practice happens in the first block or two of a row.
+// Softmax: the reference point of a row is the maximum of the first block it sees, and stays: fp32 sums and bf16 probabilities lose nothing by a
+// common factor, so nothing is compared per score.  Only when a row's sum passes 2^60 (or overflows: the first block of a row does) is the block's
+// maximum taken, the accumulators rescaled and the block's probabilities taken again -- one compare and a vote per 32-key block.
 // The table's gradient is a sum of the small differences p (dO.v - dO.o) over every pair at a distance, returned in fp32: an o that is good to
 // bf16 only (probabilities rounded before the second product, output rounded after it) would show in its third digit.  A training forward with
 // a table therefore carries the probabilities as two bf16 terms through the second product and keeps what rounding cut off the output (o_lo):
@@ -118,7 +119,7 @@ __device__ __forceinline__ void fill_gap(const int* cu, const int* len, int nd, 
 // ------------------------------------------------------------------------------------------------ scores
 
 // One block of 32 rows x 32 columns of scores, 16 of them in a lane: distance (key - query position) of register r is  rel + SGN reg_off(r).
-//   z[r]: capped score, t[r]: z plus the part of the bias that differs between registers, c: the part that does not (per lane); log2 domain.
+// The score of register r (log2 domain) is x[r] + c: c = offset() is the part of the bias that a block's registers share.
 //   lo: smallest distance of the block's first row to its columns, so that the block spans distances lo - 31 .. lo + 31
 template <int BIAS, bool CAP, int SGN> struct Scorer {
     float sc2; Cap cp;
@@ -133,36 +134,38 @@ template <int BIAS, bool CAP, int SGN> struct Scorer {
             for (int r = 0; r < 16; ++r) rc[r] = uniform_f(sl2 * (float)reg_off(r));
         }
     }
-    __device__ __forceinline__ void block(f32x16& z, float (&t)[16], float& c, int rel, int lo) const {
+    __device__ __forceinline__ float offset(int rel, int lo) const {
+        if (BIAS == 1) return lo + 31 <= 0 ? sl2 * (float)rel : lo - 31 >= 0 ? -sl2 * (float)rel : 0.f;
+        if (BIAS == 2) return lo + 31 <= -R ? far_lo : lo - 31 >= R ? far_hi : 0.f;
+        return 0.f;
+    }
+    // x[r] = score - c - mo[r]; z: the capped product, which the backward needs again (left as it was without a cap)
+    template <class M> __device__ __forceinline__ void args(f32x16& z, float (&x)[16], int rel, int lo, M&& mo) const {
         if (CAP) cap16(z, cp);
-        c = 0.f;
         const float f = CAP ? 1.f : sc2;
         if (BIAS == 0) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) t[r] = z[r] * f;
+            for (int r = 0; r < 16; ++r) x[r] = fmaf(z[r], f, -mo(r));
         } else if (BIAS == 1) {
             if (lo + 31 <= 0) {
-                c = sl2 * (float)rel;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) t[r] = fmaf(z[r], f, SGN * rc[r]);
+                for (int r = 0; r < 16; ++r) x[r] = fmaf(z[r], f, SGN * rc[r]) - mo(r);
             } else if (lo - 31 >= 0) {
-                c = -sl2 * (float)rel;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) t[r] = fmaf(z[r], f, -SGN * rc[r]);
+                for (int r = 0; r < 16; ++r) x[r] = fmaf(z[r], f, -SGN * rc[r]) - mo(r);
             } else {
                 const float d = (float)rel;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) t[r] = fmaf(-sl2, fabsf(d + (float)(SGN * reg_off(r))), z[r] * f);
+                for (int r = 0; r < 16; ++r) x[r] = fmaf(-sl2, fabsf(d + (float)(SGN * reg_off(r))), fmaf(z[r], f, -mo(r)));
             }
         } else {
             if (lo + 31 <= -R || lo - 31 >= R) {
-                c = lo < 0 ? far_lo : far_hi;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) t[r] = z[r] * f;
+                for (int r = 0; r < 16; ++r) x[r] = fmaf(z[r], f, -mo(r));
             } else {
                 const float* l = lut + PADL + R + rel;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) t[r] = fmaf(z[r], f, l[SGN * reg_off(r)]);
+                for (int r = 0; r < 16; ++r) x[r] = fmaf(z[r], f, l[SGN * reg_off(r)]) - mo(r);
             }
         }
     }
@@ -238,7 +241,7 @@ __global__ __launch_bounds__(256, 4) void pa_fwd_kernel(PAArgs p) {
     sg.init(wave, lane, p.sk, p.sv);
     int foff[4];
     frag_offsets(l31, hi, foff);
-    const TrOff tro = tr_offsets(lane);
+    const TrAddr tra = tr_addr(smem, lane);
     const bf16_t* Kb = p.K + (long)D.k0 * p.sk + (long)(h / p.G) * p.hk;
     const bf16_t* Vb = p.V + (long)D.k0 * p.sv + (long)(h / p.G) * p.hv;
 
@@ -255,69 +258,107 @@ __global__ __launch_bounds__(256, 4) void pa_fwd_kernel(PAArgs p) {
         // (every ordinary load of the prologue is waited for before the first LDS-DMA: vmcnt is counted in order)
         asm volatile("" ::"v"(qf[0]), "v"(qf[1]), "v"(qf[2]), "v"(qf[3]));
         if (nt > 0) sg.issue(Kb, Vb, D.nk - 1, smem);
-        for (int kt = 0; kt < nt; ++kt) {
+        const int qp = q0 + D.off;
+        // probabilities (arguments of exp2 in x) packed, the row's sum with them (training with a table: fp32 sums and a second term)
+        auto probs = [&](float (&x)[16], bf16x8 (&pf)[2], bf16x8 (&pl)[2], float& la, float& lb) __attribute__((always_inline)) {
+            la = l0;
+            lb = l1;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[r] = fast_exp2(x[r]);
+            pf[0] = pack8f(x);
+            pf[1] = pack8f(x + 8);
+            if (TR == 2) {
+#pragma unroll
+                for (int r = 0; r < 16; r += 2) {
+                    la += x[r];
+                    lb += x[r + 1];
+                }
+#pragma unroll
+                for (int s2 = 0; s2 < 2; ++s2) {
+                    float w[8];
+                    unpack8(__builtin_bit_cast(u32x4, pf[s2]), w);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) w[e] = x[8 * s2 + e] - w[e];
+                    pl[s2] = pack8f(w);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    la = add_bf16_pair(__builtin_bit_cast(u32x4, pf[0])[i], la);
+                    lb = add_bf16_pair(__builtin_bit_cast(u32x4, pf[1])[i], lb);
+                }
+            }
+        };
+        auto step = [&](auto stage_, int kt) __attribute__((always_inline)) {
+            constexpr int S = decltype(stage_)::value * STAGE;
             const int k0 = kt * 64;
             wait_vmcnt<0>();              // tile kt has landed for this wave ...
             barrier_raw();                // ... and for every wave; everyone is done with tile kt - 1
-            if (kt + 1 < nt) sg.issue(Kb + (long)(k0 + 64) * p.sk, Vb + (long)(k0 + 64) * p.sv, D.nk - 1 - (k0 + 64), smem + ((kt + 1) & 1) * STAGE);
-            const unsigned char* Kt = smem + (kt & 1) * STAGE;
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
+            if (kt + 1 < nt) sg.issue(Kb + (long)(k0 + 64) * p.sk, Vb + (long)(k0 + 64) * p.sv, D.nk - 1 - (k0 + 64), smem + (STAGE - S));
+            auto block = [&](auto kb_) __attribute__((always_inline)) {
+                constexpr int kb = decltype(kb_)::value;
                 const int kk = k0 + 32 * kb;
-                if (kk >= lim_hi) continue;                   // (wave-uniform) nothing of the block is visible
+                if (kk >= lim_hi) return;                     // (wave-uniform) nothing of the block is visible
                 f32x16 s = zero16();
 #pragma unroll
-                for (int ks = 0; ks < 4; ++ks) s = mfma32(ld<bf16x8>(Kt + foff[ks] + kb * 4096), qf[ks], s);
-                float t[16], c;
-                const int qp = q0 + D.off;
-                sc.block(s, t, c, kk + 8 * hi - (qp + l31), kk - qp);
-                if (kk + 32 > lim_lo) {                       // some query of the wave does not see all of the block
-                    cold_path();
-                    const int n = lim - (kk + 8 * hi);
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) t[r] = reg_off(r) < n ? t[r] : -__builtin_inff();
+                for (int ks = 0; ks < 4; ++ks) s = mfma32(ld<bf16x8>(smem + foff[ks] + (S + kb * 4096)), qf[ks], s);
+                float la, lb;
+                bf16x8 pf[2], pl[2];
+                const int rel = kk + 8 * hi - (qp + l31), lo = kk - qp;
+                bool done = false;
+                if (kk + 32 <= lim_lo) {                      // every query of the wave sees all of the block
+                    float x[16];
+                    f32x16 z = s;
+                    const float mo = m - sc.offset(rel, lo);
+                    sc.args(z, x, rel, lo, [&](int) { return mo; });
+                    probs(x, pf, pl, la, lb);
+                    done = wave_all(la + lb < L_MAX);
                 }
-                float mx = t[0];
-#pragma unroll
-                for (int r = 1; r < 16; ++r) mx = fmaxf(mx, t[r]);
-                mx += c;
-                if (!wave_all(mx <= m + M_SLACK)) {
+                if (!done) {                                  // a masked block, or a row whose sum outgrew its reference point
                     cold_path();
+                    float x[16];
+                    pin_vgpr(s);                                          // (its arithmetic is not shared with the path above: that would keep 32 registers alive)
+                    const float c = sc.offset(rel, lo);
+                    sc.args(s, x, rel, lo, [](int) { return 0.f; });
+                    const int n = lim - (kk + 8 * hi);
+                    float mx = -__builtin_inff();
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        x[r] = reg_off(r) < n ? x[r] : -__builtin_inff();
+                        mx = fmaxf(mx, x[r]);
+                    }
+                    mx += c;
                     const float mn = fmaxf(m, fmaxf(mx, lane32_other(mx))), al = fast_exp2(m - mn);
                     l0 *= al;
                     l1 *= al;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) { o[0][r] *= al; o[1][r] *= al; }
                     m = mn;
-                }
-                const float mo = m - c;
 #pragma unroll
-                for (int r = 0; r < 16; r += 2) {
-                    t[r] = fast_exp2(t[r] - mo);
-                    t[r + 1] = fast_exp2(t[r + 1] - mo);
-                    l0 += t[r];
-                    l1 += t[r + 1];
+                    for (int r = 0; r < 16; ++r) x[r] -= mn - c;
+                    probs(x, pf, pl, la, lb);
                 }
-                const bf16x8 pf[2] = {pack8f(t), pack8f(t + 8)};
+                l0 = la;
+                l1 = lb;
                 bf16x8 vf[2][2];
-                tr_frags(vf, Kt + 8192 + kb * 4096, tro);
+                tr_frags<S + 8192 + kb * 4096>(vf, tra);
 #pragma unroll
                 for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
                     for (int db = 0; db < 2; ++db) o[db] = mfma32(vf[s2][db], pf[s2], o[db]);
                 if (TR == 2) {
 #pragma unroll
-                    for (int s2 = 0; s2 < 2; ++s2) {
-                        float w[8];
-                        unpack8(__builtin_bit_cast(u32x4, pf[s2]), w);
+                    for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) w[e] = t[8 * s2 + e] - w[e];
-                        const bf16x8 pl = pack8f(w);
-#pragma unroll
-                        for (int db = 0; db < 2; ++db) o[db] = mfma32(vf[s2][db], pl, o[db]);
-                    }
+                        for (int db = 0; db < 2; ++db) o[db] = mfma32(vf[s2][db], pl[s2], o[db]);
                 }
-            }
+            };
+            block(Int<0>{});
+            block(Int<1>{});
+        };
+        for (int kt = 0; kt < nt; kt += 2) {
+            step(Int<0>{}, kt);
+            if (kt + 1 < nt) step(Int<1>{}, kt + 1);
         }
         if (live) {
             float l = l0 + l1;
@@ -423,7 +464,7 @@ __global__ __launch_bounds__(256, RG > 128 ? 2 : 3) void pa_dq_kernel(PAArgs p) 
     sg.init(wave, lane, p.sk, p.sv);
     int foff[4];
     frag_offsets(l31, hi, foff);
-    const TrOff tro = tr_offsets(lane);
+    const TrAddr tra = tr_addr(smem, lane);
     const bf16_t* Kb = p.K + (long)D.k0 * p.sk + (long)(h / p.G) * p.hk;
     const bf16_t* Vb = p.V + (long)D.k0 * p.sv + (long)(h / p.G) * p.hv;
 
@@ -458,34 +499,34 @@ __global__ __launch_bounds__(256, RG > 128 ? 2 : 3) void pa_dq_kernel(PAArgs p) 
         f32x16 dq[2] = {zero16(), zero16()};
         asm volatile("" ::"v"(qf[0]), "v"(qf[1]), "v"(qf[2]), "v"(qf[3]), "v"(dof[0]), "v"(dof[1]), "v"(dof[2]), "v"(dof[3]), "v"(lse), "v"(dl));
         if (nt > 0) sg.issue(Kb, Vb, D.nk - 1, smem);
-        for (int kt = 0; kt < nt; ++kt) {
+        auto step = [&](auto stage_, int kt) __attribute__((always_inline)) {
+            constexpr int S = decltype(stage_)::value * STAGE;
             const int k0 = kt * 64;
             wait_vmcnt<0>();
             barrier_raw();
-            if (kt + 1 < nt) sg.issue(Kb + (long)(k0 + 64) * p.sk, Vb + (long)(k0 + 64) * p.sv, D.nk - 1 - (k0 + 64), smem + ((kt + 1) & 1) * STAGE);
-            const unsigned char* Kt = smem + (kt & 1) * STAGE;
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
+            if (kt + 1 < nt) sg.issue(Kb + (long)(k0 + 64) * p.sk, Vb + (long)(k0 + 64) * p.sv, D.nk - 1 - (k0 + 64), smem + (STAGE - S));
+            auto block = [&](auto kb_) __attribute__((always_inline)) {
+                constexpr int kb = decltype(kb_)::value;
                 const int kk = k0 + 32 * kb;
-                if (kk >= lim_hi) continue;
+                if (kk >= lim_hi) return;
                 f32x16 s = zero16(), dp = zero16();
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks) {
-                    s = mfma32(ld<bf16x8>(Kt + foff[ks] + kb * 4096), qf[ks], s);
-                    dp = mfma32(ld<bf16x8>(Kt + 8192 + foff[ks] + kb * 4096), dof[ks], dp);
+                    s = mfma32(ld<bf16x8>(smem + foff[ks] + (S + kb * 4096)), qf[ks], s);
+                    dp = mfma32(ld<bf16x8>(smem + foff[ks] + (S + 8192 + kb * 4096)), dof[ks], dp);
                 }
-                float t[16], c;
-                const int qp = q0 + D.off, lo = kk - qp;
-                sc.block(s, t, c, kk + 8 * hi - (qp + l31), lo);
+                float t[16];
+                const int qp = q0 + D.off, lo = kk - qp, rel = kk + 8 * hi - (qp + l31);
+                const float mo = lse - sc.offset(rel, lo);
+                sc.args(s, t, rel, lo, [&](int) { return mo; });
                 if (kk + 32 > lim_lo) {
                     cold_path();
                     const int n = lim - (kk + 8 * hi);
 #pragma unroll
                     for (int r = 0; r < 16; ++r) t[r] = reg_off(r) < n ? t[r] : -__builtin_inff();
                 }
-                const float mo = lse - c;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) t[r] = fast_exp2(t[r] - mo) * (dp[r] - dl);       // dS
+                for (int r = 0; r < 16; ++r) t[r] = fast_exp2(t[r]) * (dp[r] - dl);            // dS
                 if (RG) {
                     if (lo + 31 <= -p.R || lo - 31 >= p.R) {
                         float a = 0.f;
@@ -505,12 +546,18 @@ __global__ __launch_bounds__(256, RG > 128 ? 2 : 3) void pa_dq_kernel(PAArgs p) 
                 }
                 const bf16x8 df[2] = {pack8f(t), pack8f(t + 8)};
                 bf16x8 kf[2][2];
-                tr_frags(kf, Kt + kb * 4096, tro);
+                tr_frags<S + kb * 4096>(kf, tra);
 #pragma unroll
                 for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
                     for (int db = 0; db < 2; ++db) dq[db] = mfma32(kf[s2][db], df[s2], dq[db]);
-            }
+            };
+            block(Int<0>{});
+            block(Int<1>{});
+        };
+        for (int kt = 0; kt < nt; kt += 2) {
+            step(Int<0>{}, kt);
+            if (kt + 1 < nt) step(Int<1>{}, kt + 1);
         }
         if (live) {
             bf16_t* drow = p.dQ + ((long)row * p.H + h) * DH;
@@ -606,7 +653,7 @@ __global__ __launch_bounds__(256, 2) void pa_dkv_kernel(PAArgs p) {
     sg.init(wave, lane, p.sq, p.sg);
     int foff[4];
     frag_offsets(l31, hi, foff);
-    const TrOff tro = tr_offsets(lane);
+    const TrAddr tra = tr_addr(smem, lane);
     const float icl = CAP ? 1.f / (p.cap * LOG2E) : 0.f;
     const int nqt = (D.nq + 63) / 64;
 
@@ -640,7 +687,8 @@ __global__ __launch_bounds__(256, 2) void pa_dkv_kernel(PAArgs p) {
         }
         asm volatile("" ::"v"(kf[0]), "v"(kf[1]), "v"(kf[2]), "v"(kf[3]), "v"(vf[0]), "v"(vf[1]), "v"(vf[2]), "v"(vf[3]));
         if (total > 0) issue(0);
-        for (int it = 0; it < total; ++it) {
+        auto step = [&](auto stage_, int it) __attribute__((always_inline)) {
+            constexpr int S = decltype(stage_)::value * KSTAGE;
             const int hd = ch, j0 = cq, q0 = (t0 + j0) * 64;
             if (++cq == per) { cq = 0; ++ch; }
             wait_vmcnt<0>();
@@ -658,37 +706,39 @@ __global__ __launch_bounds__(256, 2) void pa_dkv_kernel(PAArgs p) {
                     wait_lgkm0();
                 }
             }
-            if (!live) continue;
-            const unsigned char* Qt = smem + (it & 1) * KSTAGE;
-            const float* lse_s = (const float*)(Qt + STAGE);
-#pragma unroll
-            for (int qb = 0; qb < 2; ++qb) {
+            if (!live) return;
+            const float* lse_s = (const float*)(smem + (S + STAGE));
+            auto block = [&](auto qb_) __attribute__((always_inline)) {
+                constexpr int qb = decltype(qb_)::value;
                 const int qq = q0 + 32 * qb;                  // first query of the block
-                if (qq >= D.nq || D.lim(min(qq + 31, D.nq - 1)) <= kk) continue;
+                if (qq >= D.nq || D.lim(min(qq + 31, D.nq - 1)) <= kk) return;
                 f32x16 s = zero16(), dp = zero16();
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks) {
-                    s = mfma32(ld<bf16x8>(Qt + foff[ks] + qb * 4096), kf[ks], s);
-                    dp = mfma32(ld<bf16x8>(Qt + 8192 + foff[ks] + qb * 4096), vf[ks], dp);
+                    s = mfma32(ld<bf16x8>(smem + foff[ks] + (S + qb * 4096)), kf[ks], s);
+                    dp = mfma32(ld<bf16x8>(smem + foff[ks] + (S + 8192 + qb * 4096)), vf[ks], dp);
                 }
-                float t[16], c;
-                const int qp = qq + D.off;
-                sc.block(s, t, c, key - (qp + 8 * hi), kk - qp);
+                float t[16], ds[16];
+                const int qp = qq + D.off, lo = kk - qp, rel = key - (qp + 8 * hi);
+                const float c = sc.offset(rel, lo);
+                const float* ls = lse_s + 32 * qb + 8 * hi;
+                f32x4 l4[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) l4[i] = ld<f32x4>(ls + reg_off(4 * i));
+                sc.args(s, t, rel, lo, [&](int r) { return BIAS == 0 ? l4[r >> 2][r & 3] : l4[r >> 2][r & 3] - c; });
                 if (D.lim(qq) < kk + 32 || qq + 32 > D.nq) {
                     cold_path();
                     const int a = qmin - (qq + 8 * hi), b = D.nq - (qq + 8 * hi);
 #pragma unroll
                     for (int r = 0; r < 16; ++r) t[r] = (reg_off(r) >= a && reg_off(r) < b) ? t[r] : -__builtin_inff();
                 }
-                const float* ls = lse_s + 32 * qb + 8 * hi;
-                float ds[16];
 #pragma unroll
-                for (int r4 = 0; r4 < 16; r4 += 4) {
-                    const f32x4 l4 = ld<f32x4>(ls + reg_off(r4)), d4 = ld<f32x4>(ls + 64 + reg_off(r4));
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 d4 = ld<f32x4>(ls + 64 + reg_off(4 * i));
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const int r = r4 + j;
-                        t[r] = fast_exp2(t[r] - (BIAS == 0 ? l4[j] : l4[j] - c));
+                        const int r = 4 * i + j;
+                        t[r] = fast_exp2(t[r]);
                         ds[r] = t[r] * (dp[r] - d4[j]);
                         if (CAP) {
                             const float th = s[r] * icl;
@@ -697,19 +747,25 @@ __global__ __launch_bounds__(256, 2) void pa_dkv_kernel(PAArgs p) {
                     }
                 }
                 bf16x8 f[2][2];
-                tr_frags(f, Qt + 8192 + qb * 4096, tro);
+                tr_frags<S + 8192 + qb * 4096>(f, tra);
                 const bf16x8 pf[2] = {pack8f(t), pack8f(t + 8)};
 #pragma unroll
                 for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
                     for (int db = 0; db < 2; ++db) dv[db] = mfma32(f[s2][db], pf[s2], dv[db]);
-                tr_frags(f, Qt + qb * 4096, tro);
+                tr_frags<S + qb * 4096>(f, tra);
                 const bf16x8 df[2] = {pack8f(ds), pack8f(ds + 8)};
 #pragma unroll
                 for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
                     for (int db = 0; db < 2; ++db) dk[db] = mfma32(f[s2][db], df[s2], dk[db]);
-            }
+            };
+            block(Int<0>{});
+            block(Int<1>{});
+        };
+        for (int it = 0; it < total; it += 2) {
+            step(Int<0>{}, it);
+            if (it + 1 < total) step(Int<1>{}, it + 1);
         }
         if (live) {
             const long orow = ((long)(D.k0 + (kin ? key : 0)) * p.Hkv + wk.h) * DH;

@@ -32,10 +32,20 @@ inline s16x4_ lds_read_tr16_b64(const void* lds_ptr) {
 inline void lds_tr_issue(s16x4_& dst, const void* lds_ptr, int imm_off) { dst = lds_read_tr16_b64((const char*)lds_ptr + imm_off); }
 template <class... T> inline void lds_tr_wait(T&...) {}
 
-template <int STEP>
-inline void lds_tr_read8(s16x4_ (&d)[8], const void* lo0, const void* hi0, const void* lo1, const void* hi1) {
-    const void* a[4] = {lo0, hi0, lo1, hi1};
-    for (int i = 0; i < 8; ++i) d[i] = lds_read_tr16_b64((const char*)a[i & 3] + (i >> 2) * STEP);
+// LDS "addresses" of the model: offsets into the array that lds_declare named
+inline thread_local const char* g_lds_lo = nullptr;
+inline thread_local const char* g_lds_hi = nullptr;
+inline unsigned lds_addr(const void* p) { return (unsigned)((const char*)p - g_lds_lo); }
+template <int OFF, int STEP>
+inline void lds_tr_read8(s16x4_ (&d)[8], unsigned lo0, unsigned hi0, unsigned lo1, unsigned hi1) {
+    const unsigned a[4] = {lo0, hi0, lo1, hi1};
+    for (int i = 0; i < 8; ++i) d[i] = lds_read_tr16_b64(g_lds_lo + a[i & 3] + OFF + (i >> 2) * STEP);
+}
+inline float add_bf16_pair(unsigned pair, float acc) {
+    unsigned lo = pair << 16, hi = pair & 0xffff0000u;
+    float a, b;
+    memcpy(&a, &lo, 4); memcpy(&b, &hi, 4);
+    return acc + (a + b);
 }
 
 inline float uniform_f(float v) { return v; }
@@ -149,8 +159,6 @@ inline void order_memory() {}
 
 // the static LDS array the calling kernel's LDS-DMA copies must land in (set by lds_declare at kernel entry; a block's
 // fibers all run on one host thread, and so do its `static thread_local` __shared__ arrays)
-inline thread_local const char* g_lds_lo = nullptr;
-inline thread_local const char* g_lds_hi = nullptr;
 inline void lds_declare(const void* base, unsigned bytes) { g_lds_lo = (const char*)base; g_lds_hi = g_lds_lo + bytes; }
 inline void lds_check(const void* dst, int n) {
     if (g_lds_lo == nullptr || (const char*)dst < g_lds_lo || (const char*)dst + n > g_lds_hi) {
