@@ -39,6 +39,7 @@ using namespace e2k;
 namespace {
 
 constexpr int STAGE = 16384;          // one ring stage: two [64][64] bf16 tiles
+constexpr int NST = 3;                // ring stages: two tiles in flight while one is computed
 constexpr float LSE_EMPTY = 1e30f;    // log-sum-exp of a row that sees nothing: exp2(t - it) is 0
 constexpr int PADL = 64;              // entries of the distance table beyond its reach on either side (a block's distances spread over 63)
 constexpr int REACH_MAX = 512;
@@ -213,8 +214,8 @@ struct Stager {
 // flight while this one is computed, one raw barrier a tile).
 // TR: 0 inference, 1 training (log-sum-exps), 2 training with the table's gradient to come (two-term probabilities, o_lo)
 template <int BIAS, bool CAP, int TR>
-__global__ __launch_bounds__(256, 4) void pa_fwd_kernel(PAArgs p) {
-    __shared__ __attribute__((aligned(16))) unsigned char smem[2 * STAGE];
+__global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
+    __shared__ __attribute__((aligned(16))) unsigned char smem[NST * STAGE];
     __shared__ float lut[BIAS == 2 ? 2 * REACH_MAX + 1 + 2 * PADL : 1];
     lds_declare(smem, sizeof(smem));
     if ((int)blockIdx.x >= p.nwork) {
@@ -248,16 +249,21 @@ __global__ __launch_bounds__(256, 4) void pa_fwd_kernel(PAArgs p) {
     for (int tile = wk.tile; tile * 128 < D.nq; tile += p.nt) {
         const int q0 = tile * 128 + wave * 32, q = q0 + l31;
         const bool live = q0 < D.nq, qin = q < D.nq;
-        const int lim = qin ? D.lim(q) : 0;
+        const int qc = min(q, D.nq - 1);              // (lanes past the end repeat the last query: their sums stay in step with the wave's)
+        const int lim = D.lim(qc);
         const int lim_lo = live ? D.lim(q0) : 0, lim_hi = live ? D.lim(min(q0 + 31, D.nq - 1)) : 0;
         const int kend = D.lim(min(tile * 128 + 127, D.nq - 1)), nt = (kend + 63) / 64;
         bf16x8 qf[4];
-        row_frags(qf, p.Q + (long)(D.q0 + (qin ? q : 0)) * p.sq + (long)h * p.hq, qin, hi);
+        row_frags(qf, p.Q + (long)(D.q0 + qc) * p.sq + (long)h * p.hq, live, hi);
         f32x16 o[2] = {zero16(), zero16()};
         float m = M_INIT, l0 = 0.f, l1 = 0.f;
         // (every ordinary load of the prologue is waited for before the first LDS-DMA: vmcnt is counted in order)
         asm volatile("" ::"v"(qf[0]), "v"(qf[1]), "v"(qf[2]), "v"(qf[3]));
-        if (nt > 0) sg.issue(Kb, Vb, D.nk - 1, smem);
+        auto fetch = [&](int kt, unsigned char* S) __attribute__((always_inline)) {
+            sg.issue(Kb + (long)(kt * 64) * p.sk, Vb + (long)(kt * 64) * p.sv, D.nk - 1 - kt * 64, S);
+        };
+        if (nt > 0) fetch(0, smem);
+        if (nt > 1) fetch(1, smem + STAGE);
         const int qp = q0 + D.off;
         // probabilities (arguments of exp2 in x) packed, the row's sum with them (training with a table: fp32 sums and a second term)
         auto probs = [&](float (&x)[16], bf16x8 (&pf)[2], bf16x8 (&pl)[2], float& la, float& lb) __attribute__((always_inline)) {
@@ -292,9 +298,10 @@ __global__ __launch_bounds__(256, 4) void pa_fwd_kernel(PAArgs p) {
         auto step = [&](auto stage_, int kt) __attribute__((always_inline)) {
             constexpr int S = decltype(stage_)::value * STAGE;
             const int k0 = kt * 64;
-            wait_vmcnt<0>();              // tile kt has landed for this wave ...
-            barrier_raw();                // ... and for every wave; everyone is done with tile kt - 1
-            if (kt + 1 < nt) sg.issue(Kb + (long)(k0 + 64) * p.sk, Vb + (long)(k0 + 64) * p.sv, D.nk - 1 - (k0 + 64), smem + (STAGE - S));
+            if (kt + 1 < nt) wait_vmcnt<4>();          // tile kt has landed for this wave (tile kt + 1's four copies may be in flight) ...
+            else wait_vmcnt<0>();
+            barrier_raw();                             // ... and for every wave; everyone is done with tile kt - 1, whose stage is filled next
+            if (kt + 2 < nt) fetch(kt + 2, smem + (decltype(stage_)::value + 2) % NST * STAGE);
             auto block = [&](auto kb_) __attribute__((always_inline)) {
                 constexpr int kb = decltype(kb_)::value;
                 const int kk = k0 + 32 * kb;
@@ -356,9 +363,10 @@ __global__ __launch_bounds__(256, 4) void pa_fwd_kernel(PAArgs p) {
             block(Int<0>{});
             block(Int<1>{});
         };
-        for (int kt = 0; kt < nt; kt += 2) {
+        for (int kt = 0; kt < nt; kt += NST) {
             step(Int<0>{}, kt);
             if (kt + 1 < nt) step(Int<1>{}, kt + 1);
+            if (kt + 2 < nt) step(Int<2>{}, kt + 2);
         }
         if (live) {
             float l = l0 + l1;
@@ -429,7 +437,7 @@ constexpr int distn(int reach) { return 2 * reach + 1 + 2 * PADL; }
 // RG: 0 no table gradient, else the largest reach of this instantiation (its LDS)
 template <int BIAS, bool CAP, int RG>
 __global__ __launch_bounds__(256, RG > 128 ? 2 : 3) void pa_dq_kernel(PAArgs p) {
-    __shared__ __attribute__((aligned(16))) unsigned char smem[2 * STAGE];
+    __shared__ __attribute__((aligned(16))) unsigned char smem[NST * STAGE];
     __shared__ float lut[BIAS == 2 ? distn(RG && RG < REACH_MAX ? RG : REACH_MAX) : 1];
     __shared__ float dist[RG ? 4 * distn(RG) : 1];
     __shared__ float scr[RG ? 4 * 16 * 33 : 1];
@@ -498,13 +506,18 @@ __global__ __launch_bounds__(256, RG > 128 ? 2 : 3) void pa_dq_kernel(PAArgs p) 
         if (!qin) dl = 0.f;
         f32x16 dq[2] = {zero16(), zero16()};
         asm volatile("" ::"v"(qf[0]), "v"(qf[1]), "v"(qf[2]), "v"(qf[3]), "v"(dof[0]), "v"(dof[1]), "v"(dof[2]), "v"(dof[3]), "v"(lse), "v"(dl));
-        if (nt > 0) sg.issue(Kb, Vb, D.nk - 1, smem);
+        auto fetch = [&](int kt, unsigned char* S) __attribute__((always_inline)) {
+            sg.issue(Kb + (long)(kt * 64) * p.sk, Vb + (long)(kt * 64) * p.sv, D.nk - 1 - kt * 64, S);
+        };
+        if (nt > 0) fetch(0, smem);
+        if (nt > 1) fetch(1, smem + STAGE);
         auto step = [&](auto stage_, int kt) __attribute__((always_inline)) {
             constexpr int S = decltype(stage_)::value * STAGE;
             const int k0 = kt * 64;
-            wait_vmcnt<0>();
+            if (kt + 1 < nt) wait_vmcnt<4>();
+            else wait_vmcnt<0>();
             barrier_raw();
-            if (kt + 1 < nt) sg.issue(Kb + (long)(k0 + 64) * p.sk, Vb + (long)(k0 + 64) * p.sv, D.nk - 1 - (k0 + 64), smem + (STAGE - S));
+            if (kt + 2 < nt) fetch(kt + 2, smem + (decltype(stage_)::value + 2) % NST * STAGE);
             auto block = [&](auto kb_) __attribute__((always_inline)) {
                 constexpr int kb = decltype(kb_)::value;
                 const int kk = k0 + 32 * kb;
@@ -555,9 +568,10 @@ __global__ __launch_bounds__(256, RG > 128 ? 2 : 3) void pa_dq_kernel(PAArgs p) 
             block(Int<0>{});
             block(Int<1>{});
         };
-        for (int kt = 0; kt < nt; kt += 2) {
+        for (int kt = 0; kt < nt; kt += NST) {
             step(Int<0>{}, kt);
             if (kt + 1 < nt) step(Int<1>{}, kt + 1);
+            if (kt + 2 < nt) step(Int<2>{}, kt + 2);
         }
         if (live) {
             bf16_t* drow = p.dQ + ((long)row * p.H + h) * DH;
@@ -635,7 +649,7 @@ constexpr int KSTAGE = STAGE + 512;
 
 template <int BIAS, bool CAP>
 __global__ __launch_bounds__(256, 2) void pa_dkv_kernel(PAArgs p) {
-    __shared__ __attribute__((aligned(16))) unsigned char smem[2 * KSTAGE];
+    __shared__ __attribute__((aligned(16))) unsigned char smem[NST * KSTAGE];
     __shared__ float lut[BIAS == 2 ? 2 * distn(REACH_MAX) : 1];        // two heads' tables in turn
     lds_declare(smem, sizeof(smem));
     if ((int)blockIdx.x >= p.nwork) {
@@ -673,7 +687,7 @@ __global__ __launch_bounds__(256, 2) void pa_dkv_kernel(PAArgs p) {
         auto issue = [&](int it) __attribute__((always_inline)) {
             const int h = wk.h * p.G + ih, q0 = (t0 + iq) * 64;
             if (++iq == per) { iq = 0; ++ih; }
-            unsigned char* S = smem + (it & 1) * KSTAGE;
+            unsigned char* S = smem + it % NST * KSTAGE;
             const long r = D.q0 + q0;
             sg.issue(p.Q + r * p.sq + (long)h * p.hq, p.dO + r * p.sg + (long)h * p.hg, D.nq - 1 - q0, S);
             if (wave < 2) glds4((wave == 0 ? p.lse2 : p.delta) + (long)h * p.Tq + r + min(lane, D.nq - 1 - q0), S + STAGE + wave * 256);
@@ -687,13 +701,16 @@ __global__ __launch_bounds__(256, 2) void pa_dkv_kernel(PAArgs p) {
         }
         asm volatile("" ::"v"(kf[0]), "v"(kf[1]), "v"(kf[2]), "v"(kf[3]), "v"(vf[0]), "v"(vf[1]), "v"(vf[2]), "v"(vf[3]));
         if (total > 0) issue(0);
+        if (total > 1) issue(1);
         auto step = [&](auto stage_, int it) __attribute__((always_inline)) {
             constexpr int S = decltype(stage_)::value * KSTAGE;
             const int hd = ch, j0 = cq, q0 = (t0 + j0) * 64;
             if (++cq == per) { cq = 0; ++ch; }
-            wait_vmcnt<0>();
+            // (waves 0 and 1 have five copies a tile, the others four: four may be in flight at most)
+            if (it + 1 < total) wait_vmcnt<4>();
+            else wait_vmcnt<0>();
             barrier_raw();
-            if (it + 1 < total) issue(it + 1);
+            if (it + 2 < total) issue(it + 2);
             if (BIAS == 1 && p.G > 1 && j0 == 0 && hd > 0) sc.init(p, p.slopes[wk.h * p.G + hd]);
             if (BIAS == 2) {
                 float* L = lut + (hd & 1) * distn(REACH_MAX);
@@ -763,9 +780,10 @@ __global__ __launch_bounds__(256, 2) void pa_dkv_kernel(PAArgs p) {
             block(Int<0>{});
             block(Int<1>{});
         };
-        for (int it = 0; it < total; it += 2) {
+        for (int it = 0; it < total; it += NST) {
             step(Int<0>{}, it);
             if (it + 1 < total) step(Int<1>{}, it + 1);
+            if (it + 2 < total) step(Int<2>{}, it + 2);
         }
         if (live) {
             const long orow = ((long)(D.k0 + (kin ? key : 0)) * p.Hkv + wk.h) * DH;
