@@ -58,7 +58,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_decode_kernel(DecodeArgs p) {
         qf[ks] = col ? ld<bf16x8>(p.Q + (long)b * p.qb + (long)h * p.qh + ks * 16 + hi * 8) : bf16x8{0, 0, 0, 0, 0, 0, 0, 0};
     const float sc2 = p.scale * LOG2E;
     Cap cp{};
-    if (CAP) cp = cap_of(p.scale, p.cap);
+    if (CAP) cp = cap_of<false>(p.scale, p.cap);
     const float sl2 = BIAS == 1 ? p.slopes[h] * LOG2E : 0.f;
     const float far = BIAS == 2 ? p.table[(long)clampi(p.buckets[0], 0, p.nbuckets - 1) * p.H + h] * LOG2E : 0.f;
 
@@ -79,8 +79,8 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_decode_kernel(DecodeArgs p) {
             glds16(va + ((row & 0xffffffu) * (sv & 0xffffffu) + c), S + 4096 + u * 1024);
         }
     };
-    int foff[4];
-    frag_offsets(l31, hi, foff);
+    unsigned fra[4];
+    frag_addr(ring, l31, hi, fra);
     const TrAddr tra = tr_addr(ring, lane);
     f32x16 o[2] = {zero16(), zero16()};
     float m = M_INIT, l0 = 0.f, l1 = 0.f;
@@ -94,31 +94,36 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_decode_kernel(DecodeArgs p) {
         if (blk + STAGES - 1 < b1) wait_vmcnt<8 * (STAGES - 1)>();
         else wait_vmcnt<0>();
         wave_sync();
-        const unsigned char* Kt = ring + S;
         f32x16 s = zero16();
-        bf16x8 kf[4];
-        lds_read4(kf[0], kf[1], kf[2], kf[3], Kt + foff[0], Kt + foff[1], Kt + foff[2], Kt + foff[3]);
+        bf16x8 kf[4], vf[2][2];
+        lds_read4<S>(kf, fra);
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) s = mfma32(kf[ks], qf[ks], s);
-        if (CAP) cap16(s, cp);
+        sched_fence();
+        tr_frags<S + 4096>(vf, tra);
+        sched_fence();
         const int kk = blk * 32, rel = kk + 8 * hi - (n - 1);
         float t[16], c = 0.f;
-        const float f = CAP ? 1.f : sc2;
+        auto finish = [&](auto&& add) __attribute__((always_inline)) {
+            if constexpr (CAP) {
+                cap16<false, false>(s, t, cp, add);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) t[r] = fmaf(s[r], sc2, add(r));
+            }
+        };
         if (BIAS == 1) {
             c = sl2 * (float)rel;                              // (every key lies at or before the query)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) t[r] = fmaf(s[r], f, sl2 * (float)reg_off(r));
+            finish([&](int r) { return sl2 * (float)reg_off(r); });
         } else if (BIAS == 2 && kk + 31 - (n - 1) > -p.R) {
             cold_path();                                       // the last blocks only: within the table's reach
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
+            finish([&](int r) {
                 const int d = clampi(rel + reg_off(r), -p.R, 0) + p.R;
-                t[r] = fmaf(p.table[(long)clampi(p.buckets[d], 0, p.nbuckets - 1) * p.H + h], LOG2E, s[r] * f);
-            }
+                return p.table[(long)clampi(p.buckets[d], 0, p.nbuckets - 1) * p.H + h] * LOG2E;
+            });
         } else {
             c = far;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) t[r] = s[r] * f;
+            finish([](int) { return 0.f; });
         }
         if (kk + 32 > n) {
             cold_path();
@@ -161,8 +166,6 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_decode_kernel(DecodeArgs p) {
         }
         l0 = la;
         l1 = lb;
-        bf16x8 vf[2][2];
-        tr_frags<S + 4096>(vf, tra);
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll

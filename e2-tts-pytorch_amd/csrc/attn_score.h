@@ -16,24 +16,26 @@ template <int N> struct Int { static constexpr int value = N; };
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
 __device__ __forceinline__ constexpr int reg_off(int r) { return 16 * (r >> 3) + (r & 7); }      // row of accumulator r within its block (+ 8 hi)
 
-// tanh cap:  out tanh(s kx)  with out = cap log2(e).  |s kx| <= 0.3 (a wave vote): minimax of tanh(x) / x in x^2, four terms, relative error
-// 1e-8 (below fp32's half step); beyond: 1 - 2 / (2^(2 x log2 e) + 1), absolute error 2^-22
+// tanh cap:  out tanh(s kx)  with out = cap log2(e).  |s kx| <= 0.3 (a wave vote): minimax of tanh(x) / x in x^2, relative error 1e-8 with four terms
+// (FINE: where fp32 results depend on it), 1.2e-6 with three (where probabilities are rounded to bf16: their half step is 4e-3, and the cubed error of
+// a score is below 3e-5 at any cap up to 50); beyond: 1 - 2 / (2^(2 x log2 e) + 1), absolute error 2^-22
 constexpr float CAP_POLY_MAX = 0.3f;
 struct Cap { float a0, a1, a2, a3, k2, out, lim; };
-__device__ __forceinline__ Cap cap_of(float scale, float cap) {
+template <bool FINE> __device__ __forceinline__ Cap cap_of(float scale, float cap) {
     Cap c;
     const float kx = scale / cap, k2 = kx * kx;
     c.out = cap * LOG2E;
     const float k1 = c.out * kx;
-    c.a0 = k1;
-    c.a1 = k1 * k2 * -0.33332962f;
-    c.a2 = k1 * k2 * k2 * 0.13312598f;
-    c.a3 = k1 * k2 * k2 * k2 * -0.050222438f;
+    c.a0 = FINE ? k1 : k1 * 0.99999887f;
+    c.a1 = k1 * k2 * (FINE ? -0.33332962f : -0.33310023f);
+    c.a2 = k1 * k2 * k2 * (FINE ? 0.13312598f : 0.12633947f);
+    c.a3 = FINE ? k1 * k2 * k2 * k2 * -0.050222438f : 0.f;
     c.k2 = 2.f * LOG2E * kx;
     c.lim = CAP_POLY_MAX / kx;
     return c;
 }
-__device__ __forceinline__ void cap16(f32x16& z, const Cap& cp) {
+// x[r] = capped z[r] + add(r), and with KEEP z[r] capped in place (the backward's 1 - tanh^2)
+template <bool FINE, bool KEEP, class A> __device__ __forceinline__ void cap16(f32x16& z, float (&x)[16], const Cap& cp, A&& add) {
     float a = 0.f;
 #pragma unroll
     for (int r = 0; r < 16; r += 2) a = fmaxf(fmaxf(fabsf(z[r]), fabsf(z[r + 1])), a);
@@ -41,12 +43,22 @@ __device__ __forceinline__ void cap16(f32x16& z, const Cap& cp) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const float w = z[r] * z[r];
-            z[r] *= fmaf(fmaf(fmaf(w, cp.a3, cp.a2), w, cp.a1), w, cp.a0);
+            const float u = fmaf(FINE ? fmaf(fmaf(w, cp.a3, cp.a2), w, cp.a1) : fmaf(w, cp.a2, cp.a1), w, cp.a0);
+            if (KEEP) {
+                z[r] *= u;
+                x[r] = z[r] + add(r);
+            } else {
+                x[r] = fmaf(z[r], u, add(r));
+            }
         }
     } else {
         cold_path();
 #pragma unroll
-        for (int r = 0; r < 16; ++r) z[r] = fmaf(-2.f * cp.out, fast_rcp(fast_exp2(z[r] * cp.k2) + 1.f), cp.out);
+        for (int r = 0; r < 16; ++r) {
+            const float c = fmaf(-2.f * cp.out, fast_rcp(fast_exp2(z[r] * cp.k2) + 1.f), cp.out);
+            if (KEEP) z[r] = c;
+            x[r] = c + add(r);
+        }
     }
 }
 
@@ -62,6 +74,14 @@ template <int OFF> __device__ __forceinline__ void tr_frags(bf16x8 (&f)[2][2], c
     lds_tr_read8<OFF, 2048>(d, t.lo[0], t.hi_[0], t.lo[1], t.hi_[1]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i >> 1][i & 1] = __builtin_shufflevector(d[2 * i], d[2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// addresses of a lane's row fragments (frag_offsets) in the tile image at `tile`
+__device__ __forceinline__ void frag_addr(const unsigned char* tile, int l31, int hi, unsigned (&a)[4]) {
+    int off[4];
+    frag_offsets(l31, hi, off);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) a[j] = lds_addr(tile + off[j]);
 }
 
 __device__ __forceinline__ f32x16 zero16() {

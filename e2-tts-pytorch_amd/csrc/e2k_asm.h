@@ -58,15 +58,22 @@ __device__ __forceinline__ float add_bf16_pair(unsigned pair, float acc) {
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, pair), __builtin_bit_cast(b2, 0x3f803f80u), acc, false);
 }
 
-// Four 16-byte LDS reads and their wait in one statement, for a kernel whose LDS-DMA copies into the next ring stage must stay in flight across
-// them (before its own ds_reads the compiler waits for every copy when it cannot tell the stages apart).
-__device__ __forceinline__ void lds_read4(bf16x8_& r0, bf16x8_& r1, bf16x8_& r2, bf16x8_& r3, const void* p0, const void* p1, const void* p2, const void* p3) {
-    typedef const __attribute__((address_space(3))) void* lp_t;
-    const unsigned a0 = (unsigned)(unsigned long long)(lp_t)(p0), a1 = (unsigned)(unsigned long long)(lp_t)(p1);
-    const unsigned a2 = (unsigned)(unsigned long long)(lp_t)(p2), a3 = (unsigned)(unsigned long long)(lp_t)(p3);
+// Row fragments of a tile block: four (eight) 16-byte LDS reads at OFF (and OFF2) bytes behind the four addresses and their wait in one statement:
+// one LDS latency for all of them (left to itself the compiler reads two, waits, multiplies, reads two), and copies into another ring stage stay
+// in flight across them (before its own ds_reads the compiler waits for every LDS-DMA when it cannot tell the stages apart).
+template <int OFF> __device__ __forceinline__ void lds_read4(bf16x8_ (&r)[4], const unsigned (&a)[4]) {
     asm volatile(
-        "ds_read_b128 %0, %4\n ds_read_b128 %1, %5\n ds_read_b128 %2, %6\n ds_read_b128 %3, %7\n s_waitcnt lgkmcnt(0)"
-        : "=&v"(r0), "=&v"(r1), "=&v"(r2), "=&v"(r3) : "v"(a0), "v"(a1), "v"(a2), "v"(a3) : "memory");
+        "ds_read_b128 %0, %4 offset:%8\n ds_read_b128 %1, %5 offset:%8\n ds_read_b128 %2, %6 offset:%8\n ds_read_b128 %3, %7 offset:%8\n"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]) : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(OFF) : "memory");
+}
+template <int OFF, int OFF2> __device__ __forceinline__ void lds_read8(bf16x8_ (&r)[4], bf16x8_ (&q)[4], const unsigned (&a)[4]) {
+    asm volatile(
+        "ds_read_b128 %0, %8 offset:%12\n ds_read_b128 %4, %8 offset:%13\n ds_read_b128 %1, %9 offset:%12\n ds_read_b128 %5, %9 offset:%13\n"
+        "ds_read_b128 %2, %10 offset:%12\n ds_read_b128 %6, %10 offset:%13\n ds_read_b128 %3, %11 offset:%12\n ds_read_b128 %7, %11 offset:%13\n"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(q[0]), "=&v"(q[1]), "=&v"(q[2]), "=&v"(q[3])
+        : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(OFF), "n"(OFF2) : "memory");
 }
 
 // raw v_exp_f32 (2^x, no denormal fix-up: results below 2^-126 flush to 0) and v_rcp_f32 (1 ulp)

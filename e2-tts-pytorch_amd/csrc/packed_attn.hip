@@ -122,13 +122,13 @@ __device__ __forceinline__ void fill_gap(const int* cu, const int* len, int nd, 
 // One block of 32 rows x 32 columns of scores, 16 of them in a lane: distance (key - query position) of register r is  rel + SGN reg_off(r).
 // The score of register r (log2 domain) is x[r] + c: c = offset() is the part of the bias that a block's registers share.
 //   lo: smallest distance of the block's first row to its columns, so that the block spans distances lo - 31 .. lo + 31
-template <int BIAS, bool CAP, int SGN> struct Scorer {
+template <int BIAS, bool CAP, int SGN, bool FINE, bool KEEP> struct Scorer {
     float sc2; Cap cp;
     float sl2, rc[16];                       // BIAS 1: slope log2(e), and times reg_off(r)
     const float* lut; int R; float far_lo, far_hi;
     __device__ __forceinline__ void init(const PAArgs& p, float slope) {
         sc2 = p.scale * LOG2E;
-        if (CAP) cp = cap_of(p.scale, p.cap);
+        if (CAP) cp = cap_of<FINE>(p.scale, p.cap);
         if (BIAS == 1) {
             sl2 = uniform_f(slope * LOG2E);
 #pragma unroll
@@ -140,34 +140,27 @@ template <int BIAS, bool CAP, int SGN> struct Scorer {
         if (BIAS == 2) return lo + 31 <= -R ? far_lo : lo - 31 >= R ? far_hi : 0.f;
         return 0.f;
     }
-    // x[r] = score - c - mo[r]; z: the capped product, which the backward needs again (left as it was without a cap)
+    // x[r] = score - c - mo(r).  KEEP: z becomes the capped product, which the backward needs again (left as it was without a cap)
     template <class M> __device__ __forceinline__ void args(f32x16& z, float (&x)[16], int rel, int lo, M&& mo) const {
-        if (CAP) cap16(z, cp);
-        const float f = CAP ? 1.f : sc2;
+        auto finish = [&](auto&& add) __attribute__((always_inline)) {
+            if constexpr (CAP) {
+                cap16<FINE, KEEP>(z, x, cp, add);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[r] = fmaf(z[r], sc2, add(r));
+            }
+        };
         if (BIAS == 0) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) x[r] = fmaf(z[r], f, -mo(r));
+            finish([&](int r) { return -mo(r); });
         } else if (BIAS == 1) {
-            if (lo + 31 <= 0) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) x[r] = fmaf(z[r], f, SGN * rc[r]) - mo(r);
-            } else if (lo - 31 >= 0) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) x[r] = fmaf(z[r], f, -SGN * rc[r]) - mo(r);
-            } else {
-                const float d = (float)rel;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) x[r] = fmaf(-sl2, fabsf(d + (float)(SGN * reg_off(r))), fmaf(z[r], f, -mo(r)));
-            }
+            const float d = (float)rel;
+            if (lo + 31 <= 0) finish([&](int r) { return SGN * rc[r] - mo(r); });
+            else if (lo - 31 >= 0) finish([&](int r) { return -SGN * rc[r] - mo(r); });
+            else finish([&](int r) { return fmaf(-sl2, fabsf(d + (float)(SGN * reg_off(r))), -mo(r)); });
         } else {
-            if (lo + 31 <= -R || lo - 31 >= R) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) x[r] = fmaf(z[r], f, -mo(r));
-            } else {
-                const float* l = lut + PADL + R + rel;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) x[r] = fmaf(z[r], f, l[SGN * reg_off(r)]) - mo(r);
-            }
+            const float* l = lut + PADL + R + rel;
+            if (lo + 31 <= -R || lo - 31 >= R) finish([&](int r) { return -mo(r); });
+            else finish([&](int r) { return l[SGN * reg_off(r)] - mo(r); });
         }
     }
 };
@@ -228,7 +221,7 @@ __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
     const int h = wk.h;
     const Doc D = doc_of(p, wk.d);
     if (wk.tile * 128 >= D.nq) return;
-    Scorer<BIAS, CAP, 1> sc;
+    Scorer<BIAS, CAP, 1, TR == 2, false> sc;
     sc.init(p, BIAS == 1 ? p.slopes[h] : 0.f);
     if (BIAS == 2) {
         load_lut(p, h, lut);
@@ -240,8 +233,8 @@ __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
     }
     Stager sg;
     sg.init(wave, lane, p.sk, p.sv);
-    int foff[4];
-    frag_offsets(l31, hi, foff);
+    unsigned fra[4];
+    frag_addr(smem, l31, hi, fra);
     const TrAddr tra = tr_addr(smem, lane);
     const bf16_t* Kb = p.K + (long)D.k0 * p.sk + (long)(h / p.G) * p.hk;
     const bf16_t* Vb = p.V + (long)D.k0 * p.sv + (long)(h / p.G) * p.hv;
@@ -306,9 +299,15 @@ __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
                 constexpr int kb = decltype(kb_)::value;
                 const int kk = k0 + 32 * kb;
                 if (kk >= lim_hi) return;                     // (wave-uniform) nothing of the block is visible
+                // (the transposed V fragments are read while the score products run)
                 f32x16 s = zero16();
+                bf16x8 kf[4], vf[2][2];
+                lds_read4<S + kb * 4096>(kf, fra);
 #pragma unroll
-                for (int ks = 0; ks < 4; ++ks) s = mfma32(ld<bf16x8>(smem + foff[ks] + (S + kb * 4096)), qf[ks], s);
+                for (int ks = 0; ks < 4; ++ks) s = mfma32(kf[ks], qf[ks], s);
+                sched_fence();
+                tr_frags<S + 8192 + kb * 4096>(vf, tra);
+                sched_fence();
                 float la, lb;
                 bf16x8 pf[2], pl[2];
                 const int rel = kk + 8 * hi - (qp + l31), lo = kk - qp;
@@ -347,8 +346,6 @@ __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
                 }
                 l0 = la;
                 l1 = lb;
-                bf16x8 vf[2][2];
-                tr_frags<S + 8192 + kb * 4096>(vf, tra);
 #pragma unroll
                 for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
@@ -436,7 +433,7 @@ constexpr int distn(int reach) { return 2 * reach + 1 + 2 * PADL; }
 
 // RG: 0 no table gradient, else the largest reach of this instantiation (its LDS)
 template <int BIAS, bool CAP, int RG>
-__global__ __launch_bounds__(256, RG > 128 ? 2 : 3) void pa_dq_kernel(PAArgs p) {
+__global__ __launch_bounds__(256, (BIAS || CAP) ? 2 : 3) void pa_dq_kernel(PAArgs p) {
     __shared__ __attribute__((aligned(16))) unsigned char smem[NST * STAGE];
     __shared__ float lut[BIAS == 2 ? distn(RG && RG < REACH_MAX ? RG : REACH_MAX) : 1];
     __shared__ float dist[RG ? 4 * distn(RG) : 1];
@@ -453,7 +450,7 @@ __global__ __launch_bounds__(256, RG > 128 ? 2 : 3) void pa_dq_kernel(PAArgs p) 
     const Doc D = doc_of(p, wk.d);
     if (wk.tile * 128 >= D.nq) return;
     const int ND = 2 * p.R + 1 + 2 * PADL;
-    Scorer<BIAS, CAP, 1> sc;
+    Scorer<BIAS, CAP, 1, (RG > 0), true> sc;
     sc.init(p, BIAS == 1 ? p.slopes[h] : 0.f);
     if (BIAS == 2) {
         load_lut(p, h, lut);
@@ -470,8 +467,8 @@ __global__ __launch_bounds__(256, RG > 128 ? 2 : 3) void pa_dq_kernel(PAArgs p) 
     const float icl = CAP ? 1.f / (p.cap * LOG2E) : 0.f;
     Stager sg;
     sg.init(wave, lane, p.sk, p.sv);
-    int foff[4];
-    frag_offsets(l31, hi, foff);
+    unsigned fra[4];
+    frag_addr(smem, l31, hi, fra);
     const TrAddr tra = tr_addr(smem, lane);
     const bf16_t* Kb = p.K + (long)D.k0 * p.sk + (long)(h / p.G) * p.hk;
     const bf16_t* Vb = p.V + (long)D.k0 * p.sv + (long)(h / p.G) * p.hv;
@@ -523,11 +520,19 @@ __global__ __launch_bounds__(256, RG > 128 ? 2 : 3) void pa_dq_kernel(PAArgs p) 
                 const int kk = k0 + 32 * kb;
                 if (kk >= lim_hi) return;
                 f32x16 s = zero16(), dp = zero16();
+                bf16x8 kt_[2][2];
+                {
+                    bf16x8 kf[4], vf[4];
+                    lds_read8<S + kb * 4096, S + 8192 + kb * 4096>(kf, vf, fra);
 #pragma unroll
-                for (int ks = 0; ks < 4; ++ks) {
-                    s = mfma32(ld<bf16x8>(smem + foff[ks] + (S + kb * 4096)), qf[ks], s);
-                    dp = mfma32(ld<bf16x8>(smem + foff[ks] + (S + 8192 + kb * 4096)), dof[ks], dp);
+                    for (int ks = 0; ks < 4; ++ks) {
+                        s = mfma32(kf[ks], qf[ks], s);
+                        dp = mfma32(vf[ks], dof[ks], dp);
+                    }
                 }
+                sched_fence();
+                tr_frags<S + kb * 4096>(kt_, tra);
+                sched_fence();
                 float t[16];
                 const int qp = q0 + D.off, lo = kk - qp, rel = kk + 8 * hi - (qp + l31);
                 const float mo = lse - sc.offset(rel, lo);
@@ -558,12 +563,10 @@ __global__ __launch_bounds__(256, RG > 128 ? 2 : 3) void pa_dq_kernel(PAArgs p) 
                     }
                 }
                 const bf16x8 df[2] = {pack8f(t), pack8f(t + 8)};
-                bf16x8 kf[2][2];
-                tr_frags<S + kb * 4096>(kf, tra);
 #pragma unroll
                 for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
-                    for (int db = 0; db < 2; ++db) dq[db] = mfma32(kf[s2][db], df[s2], dq[db]);
+                    for (int db = 0; db < 2; ++db) dq[db] = mfma32(kt_[s2][db], df[s2], dq[db]);
             };
             block(Int<0>{});
             block(Int<1>{});
@@ -665,8 +668,8 @@ __global__ __launch_bounds__(256, 2) void pa_dkv_kernel(PAArgs p) {
     if (tile0 * 128 >= D.nk) return;
     Stager sg;
     sg.init(wave, lane, p.sq, p.sg);
-    int foff[4];
-    frag_offsets(l31, hi, foff);
+    unsigned fra[4];
+    frag_addr(smem, l31, hi, fra);
     const TrAddr tra = tr_addr(smem, lane);
     const float icl = CAP ? 1.f / (p.cap * LOG2E) : 0.f;
     const int nqt = (D.nq + 63) / 64;
@@ -692,7 +695,7 @@ __global__ __launch_bounds__(256, 2) void pa_dkv_kernel(PAArgs p) {
             sg.issue(p.Q + r * p.sq + (long)h * p.hq, p.dO + r * p.sg + (long)h * p.hg, D.nq - 1 - q0, S);
             if (wave < 2) glds4((wave == 0 ? p.lse2 : p.delta) + (long)h * p.Tq + r + min(lane, D.nq - 1 - q0), S + STAGE + wave * 256);
         };
-        Scorer<BIAS, CAP, -1> sc;
+        Scorer<BIAS, CAP, -1, false, true> sc;
         sc.init(p, BIAS == 1 ? p.slopes[wk.h * p.G] : 0.f);
         if (BIAS == 2) {
             sc.R = p.R;
@@ -730,11 +733,20 @@ __global__ __launch_bounds__(256, 2) void pa_dkv_kernel(PAArgs p) {
                 const int qq = q0 + 32 * qb;                  // first query of the block
                 if (qq >= D.nq || D.lim(min(qq + 31, D.nq - 1)) <= kk) return;
                 f32x16 s = zero16(), dp = zero16();
+                bf16x8 dot_[2][2], qt_[2][2];
+                {
+                    bf16x8 qf[4], gf[4];
+                    lds_read8<S + qb * 4096, S + 8192 + qb * 4096>(qf, gf, fra);
 #pragma unroll
-                for (int ks = 0; ks < 4; ++ks) {
-                    s = mfma32(ld<bf16x8>(smem + foff[ks] + (S + qb * 4096)), kf[ks], s);
-                    dp = mfma32(ld<bf16x8>(smem + foff[ks] + (S + 8192 + qb * 4096)), vf[ks], dp);
+                    for (int ks = 0; ks < 4; ++ks) {
+                        s = mfma32(qf[ks], kf[ks], s);
+                        dp = mfma32(gf[ks], vf[ks], dp);
+                    }
                 }
+                sched_fence();
+                tr_frags<S + 8192 + qb * 4096>(dot_, tra);
+                tr_frags<S + qb * 4096>(qt_, tra);
+                sched_fence();
                 float t[16], ds[16];
                 const int qp = qq + D.off, lo = kk - qp, rel = key - (qp + 8 * hi);
                 const float c = sc.offset(rel, lo);
@@ -763,19 +775,14 @@ __global__ __launch_bounds__(256, 2) void pa_dkv_kernel(PAArgs p) {
                         }
                     }
                 }
-                bf16x8 f[2][2];
-                tr_frags<S + 8192 + qb * 4096>(f, tra);
-                const bf16x8 pf[2] = {pack8f(t), pack8f(t + 8)};
+                const bf16x8 pf[2] = {pack8f(t), pack8f(t + 8)}, df[2] = {pack8f(ds), pack8f(ds + 8)};
 #pragma unroll
                 for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
-                    for (int db = 0; db < 2; ++db) dv[db] = mfma32(f[s2][db], pf[s2], dv[db]);
-                tr_frags<S + qb * 4096>(f, tra);
-                const bf16x8 df[2] = {pack8f(ds), pack8f(ds + 8)};
-#pragma unroll
-                for (int s2 = 0; s2 < 2; ++s2)
-#pragma unroll
-                    for (int db = 0; db < 2; ++db) dk[db] = mfma32(f[s2][db], df[s2], dk[db]);
+                    for (int db = 0; db < 2; ++db) {
+                        dv[db] = mfma32(dot_[s2][db], pf[s2], dv[db]);
+                        dk[db] = mfma32(qt_[s2][db], df[s2], dk[db]);
+                    }
             };
             block(Int<0>{});
             block(Int<1>{});

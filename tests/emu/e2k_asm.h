@@ -85,8 +85,12 @@ inline float fast_rcp(float x) { return 1.0f / x; }
 // host model of v_mfma_f32_32x32x16_bf16 (fragment layout: csrc/e2k_asm.h)
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short bf16x8_ __attribute__((ext_vector_type(8)));
-inline void lds_read4(bf16x8_& r0, bf16x8_& r1, bf16x8_& r2, bf16x8_& r3, const void* p0, const void* p1, const void* p2, const void* p3) {
-    memcpy(&r0, p0, 16); memcpy(&r1, p1, 16); memcpy(&r2, p2, 16); memcpy(&r3, p3, 16);
+template <int OFF> inline void lds_read4(bf16x8_ (&r)[4], const unsigned (&a)[4]) {
+    for (int i = 0; i < 4; ++i) memcpy(&r[i], g_lds_lo + a[i] + OFF, 16);
+}
+template <int OFF, int OFF2> inline void lds_read8(bf16x8_ (&r)[4], bf16x8_ (&q)[4], const unsigned (&a)[4]) {
+    lds_read4<OFF>(r, a);
+    lds_read4<OFF2>(q, a);
 }
 inline f32x16 mfma32(bf16x8_ a, bf16x8_ b, f32x16 c) {
     struct AB { bf16x8_ a, b; };
