@@ -58,6 +58,7 @@ struct PAArgs {
     bf16_t *dQ, *dK, *dV;                              // (Tq, H, 64), (Tk, Hkv, 64)
     float* dist;                                       // [workgroup of the dQ grid][2 R + 1]: sums of dS by distance
     int nt, nwork;                                     // row tiles per (document, head) of this grid; workgroups that compute
+    int splits; float* part;                           // dK / dV: parts of a key tile's sweep, their sums [part][dK | dV][Tk][Hkv][64]
 };
 
 // rows of document d, kept inside [0, total) whatever the offsets say
@@ -648,6 +649,8 @@ __global__ __launch_bounds__(256) void pa_table_grad_kernel(const float* by_dist
 // One workgroup = 128 keys of one (document, key head); sweep over the 64-query tiles of all its query heads.  The query rows of the Q / dO tiles
 // are K-type images, so the accumulators (rows = queries) are the B operands of dV^T = dO^T P and dK^T = Q^T dS; their A operands come out of the
 // same tiles by transposing reads.  The 64 lse / delta values of a query tile ride along in the ring stage.
+// Few key heads and tokens leave the chip's 512 slots for these workgroups empty: the sweep is then cut into `splits` parts whose fp32 sums a second
+// kernel adds in order (7392 tokens, 4 key heads of 16: 271 us whole, see splits_for for the rule).
 constexpr int KSTAGE = STAGE + 512;
 
 template <int BIAS, bool CAP>
@@ -662,7 +665,9 @@ __global__ __launch_bounds__(256, 2) void pa_dkv_kernel(PAArgs p) {
     }
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform_i(tid >> 6);
     const int l31 = lane & 31, hi = lane >> 5;
-    const Work wk = work_of(p);
+    Work wk = work_of(p);                          // (key head, document, tile) x part
+    const int part = wk.h % p.splits;
+    wk.h /= p.splits;
     const Doc D = doc_of(p, wk.d);
     const int tile0 = p.nt - 1 - wk.tile;          // (causal: the first keys are seen by the most queries)
     if (tile0 * 128 >= D.nk) return;
@@ -685,8 +690,9 @@ __global__ __launch_bounds__(256, 2) void pa_dkv_kernel(PAArgs p) {
         const int qmin = (!D.causal || key < D.prefix) ? -0x40000000 : key - D.off;
         int t0 = 0;
         if (D.causal && tile * 128 >= D.prefix) t0 = max(0, tile * 128 - D.off) / 64;
-        const int per = max(0, nqt - t0), total = per * p.G;
-        int ih = 0, iq = 0, ch = 0, cq = 0;          // head and tile that is fetched / computed next
+        const int per = max(0, nqt - t0), all = per * p.G;
+        const int it0 = (int)((long)all * part / p.splits), total = (int)((long)all * (part + 1) / p.splits) - it0;
+        int ih = per ? it0 / per : 0, iq = it0 - ih * per, ch = ih, cq = iq;          // head and tile that is fetched / computed next
         auto issue = [&](int it) __attribute__((always_inline)) {
             const int h = wk.h * p.G + ih, q0 = (t0 + iq) * 64;
             if (++iq == per) { iq = 0; ++ih; }
@@ -696,10 +702,10 @@ __global__ __launch_bounds__(256, 2) void pa_dkv_kernel(PAArgs p) {
             if (wave < 2) glds4((wave == 0 ? p.lse2 : p.delta) + (long)h * p.Tq + r + min(lane, D.nq - 1 - q0), S + STAGE + wave * 256);
         };
         Scorer<BIAS, CAP, -1, false, true> sc;
-        sc.init(p, BIAS == 1 ? p.slopes[wk.h * p.G] : 0.f);
+        sc.init(p, BIAS == 1 ? p.slopes[wk.h * p.G + min(ch, p.G - 1)] : 0.f);
         if (BIAS == 2) {
             sc.R = p.R;
-            if (total > 0) load_lut(p, wk.h * p.G, lut);
+            if (total > 0) load_lut(p, wk.h * p.G + ch, lut + (ch & 1) * distn(REACH_MAX));
             wait_lgkm0();
         }
         asm volatile("" ::"v"(kf[0]), "v"(kf[1]), "v"(kf[2]), "v"(kf[3]), "v"(vf[0]), "v"(vf[1]), "v"(vf[2]), "v"(vf[3]));
@@ -714,7 +720,7 @@ __global__ __launch_bounds__(256, 2) void pa_dkv_kernel(PAArgs p) {
             else wait_vmcnt<0>();
             barrier_raw();
             if (it + 2 < total) issue(it + 2);
-            if (BIAS == 1 && p.G > 1 && j0 == 0 && hd > 0) sc.init(p, p.slopes[wk.h * p.G + hd]);
+            if (BIAS == 1 && p.G > 1 && j0 == 0 && it > 0) sc.init(p, p.slopes[wk.h * p.G + hd]);
             if (BIAS == 2) {
                 float* L = lut + (hd & 1) * distn(REACH_MAX);
                 sc.lut = L;
@@ -794,22 +800,76 @@ __global__ __launch_bounds__(256, 2) void pa_dkv_kernel(PAArgs p) {
         }
         if (live) {
             const long orow = ((long)(D.k0 + (kin ? key : 0)) * p.Hkv + wk.h) * DH;
-            auto put = [&](bf16_t* dst, float f, int db, int g, int hi_, bool ok, const float* a, const float* b) __attribute__((always_inline)) {
-                float v[8];
+            if (p.splits > 1) {
+                float* ws = p.part + (long)part * 2 * p.Tk * p.Hkv * DH + orow;
+                if (kin) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) { v[e] = a[e] * f; v[4 + e] = b[e] * f; }
-                u32x2 x = pack4(v), y = pack4(v + 4);
-                swap_pair(x, y);
-                if (ok) st<u32x4>(dst + orow + 32 * db + 8 * (g + hi_), u32x4{x[0], x[1], y[0], y[1]});
-            };
-            store_rows32(dk, hi, kin, [&](int db, int g, int hi_, bool ok, const float* a, const float* b) __attribute__((always_inline)) { put(p.dK, p.scale, db, g, hi_, ok, a, b); });
-            store_rows32(dv, hi, kin, [&](int db, int g, int hi_, bool ok, const float* a, const float* b) __attribute__((always_inline)) { put(p.dV, 1.f, db, g, hi_, ok, a, b); });
+                    for (int db = 0; db < 2; ++db)
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            const int col = 32 * db + 8 * g + 4 * hi;
+                            st<f32x4>(ws + col, f32x4{dk[db][4 * g], dk[db][4 * g + 1], dk[db][4 * g + 2], dk[db][4 * g + 3]});
+                            st<f32x4>(ws + (long)p.Tk * p.Hkv * DH + col, f32x4{dv[db][4 * g], dv[db][4 * g + 1], dv[db][4 * g + 2], dv[db][4 * g + 3]});
+                        }
+                }
+            } else {
+                auto put = [&](bf16_t* dst, float f, int db, int g, int hi_, bool ok, const float* a, const float* b) __attribute__((always_inline)) {
+                    float v[8];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { v[e] = a[e] * f; v[4 + e] = b[e] * f; }
+                    u32x2 x = pack4(v), y = pack4(v + 4);
+                    swap_pair(x, y);
+                    if (ok) st<u32x4>(dst + orow + 32 * db + 8 * (g + hi_), u32x4{x[0], x[1], y[0], y[1]});
+                };
+                store_rows32(dk, hi, kin, [&](int db, int g, int hi_, bool ok, const float* a, const float* b) __attribute__((always_inline)) { put(p.dK, p.scale, db, g, hi_, ok, a, b); });
+                store_rows32(dv, hi, kin, [&](int db, int g, int hi_, bool ok, const float* a, const float* b) __attribute__((always_inline)) { put(p.dV, 1.f, db, g, hi_, ok, a, b); });
+            }
         }
         if ((tile + p.nt) * 128 < D.nk) __syncthreads();
     }
 }
 
+// dK, dV = sums of the parts; one workgroup = 32 rows of a document, eight columns a thread
+__global__ __launch_bounds__(256) void pa_dkv_join_kernel(PAArgs p) {
+    const int tile = (int)blockIdx.x % p.nt, d = (int)blockIdx.x / p.nt, w = p.Hkv * DH;
+    const Span s = span(p.cu_k, p.len_k, d, p.Tk);
+    for (int r0 = tile * 32; r0 < s.n; r0 += p.nt * 32) {
+        const int rows = min(32, s.n - r0);
+        const long base = (long)(s.at + r0) * w;
+        for (int i = threadIdx.x; i < rows * (w / 8); i += 256) {
+            const long at = base + (long)i * 8;
+            float a[8], b[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { a[e] = 0.f; b[e] = 0.f; }
+            for (int q = 0; q < p.splits; ++q) {
+                const float* x = p.part + (long)q * 2 * p.Tk * w + at;
+                const float* y = x + (long)p.Tk * w;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const f32x4 u = ld<f32x4>(x + 4 * c), v = ld<f32x4>(y + 4 * c);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { a[4 * c + e] += u[e]; b[4 * c + e] += v[e]; }
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) a[e] *= p.scale;
+            st<u32x4>(p.dK + at, pack8(a));
+            st<u32x4>(p.dV + at, pack8(b));
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ host side
+
+// Parts of a key tile's sweep: as many as bring the workgroups to twice the chip's 512 slots, at most eight, each with four query tiles or more
+int splits_for(int Tk, int H, int Hkv, int max_q, int Tq) {
+    if (max_q <= 0 || max_q > Tq) max_q = Tq;
+    const long wgs = (long)((Tk + 127) / 128) * Hkv, sweep = (long)(H / Hkv) * ((max_q + 63) / 64);
+    if (wgs < 1 || wgs >= 384) return 1;
+    long s = 1024 / wgs;
+    if (s > sweep / 4) s = sweep / 4;
+    return (int)(s < 1 ? 1 : s > 8 ? 8 : s);
+}
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 bool strides_ok(long t, long h) { return t % 8 == 0 && h % 8 == 0 && t >= 0 && h >= 0 && t < (1 << 23); }
@@ -922,23 +982,34 @@ int packed_attn_bwd_impl(const void* dO, int64_t sg, int64_t hg, const void* Q, 
     } else if (nd < 0 || Tk < 0 || H < 1 || Hkv < 1 || H % Hkv != 0) {
         return E2K_ERR_SHAPE;
     }
+    float* rest = ws;                          // workspace behind the table's part
     if (dtable) {
         if (!table || !ws || nbuckets < 1 || reach < 0 || reach > REACH_MAX) return E2K_ERR_ARG;
         const int N = 2 * reach + 1;
-        float* by_dist = ws + (Tq > 0 ? (long)a.nwork * N : 0);
+        const long nq_work = a.nwork;
+        float* by_dist = ws + (Tq > 0 ? nq_work * N : 0);
         if (Tq == 0) a.nd = 0;                 // nothing was written: the sums are empty
         hipLaunchKernelGGL(pa_dist_reduce_kernel, dim3((N + 63) / 64, H), dim3(1024), 0, st, a, by_dist);
         E2K_CHECK_LAUNCH();
         hipLaunchKernelGGL(pa_table_grad_kernel, dim3((nbuckets * H + 3) / 4), dim3(256), 0, st, by_dist, buckets, N, nbuckets, H, dtable, accumulate);
         E2K_CHECK_LAUNCH();
         a.nd = nd;
+        rest = ws + (((Tq > 0 ? (long)nq_work * N : 0) + (long)H * N + 3) / 4 * 4);          // (16-byte rows)
     }
     if (Tk > 0) {
         if (!dK || !dV || !aligned16(dK) || !aligned16(dV)) return E2K_ERR_ARG;
-        const int rg = plan_grid(a, max_k, Tk, Hkv, grid);
+        a.splits = splits_for(Tk, H, Hkv, max_q, Tq);
+        a.part = rest;
+        if (a.splits > 1 && !ws) return E2K_ERR_ARG;
+        const int rg = plan_grid(a, max_k, Tk, Hkv * a.splits, grid);
         if (rg) return rg;
         if (grid > 0) {
             PA_PICK(run_dkv, a, 0, grid, st);
+            E2K_CHECK_LAUNCH();
+        }
+        if (a.splits > 1 && a.nwork > 0) {
+            a.nt *= 4;                         // 32-row tiles
+            hipLaunchKernelGGL(pa_dkv_join_kernel, dim3((unsigned)(a.nd * a.nt)), dim3(256), 0, st, a);
             E2K_CHECK_LAUNCH();
         }
     }
@@ -957,11 +1028,15 @@ int e2k_packed_attn_fwd(const void* Q, int64_t sq, int64_t hq, const void* K, in
     return e2k::dispatch("packed_attn_fwd", packed_attn_fwd_impl, Q, sq, hq, K, sk, hk, V, sv, hv, cu_q, cu_k, len_q, len_k, prefix, nd, Tq, Tk, H, Hkv,
                          max_q, causal, scale, softcap, slopes, table, buckets, nbuckets, reach, O, so, ho, Olo, lse2, fill_gaps, stream);
 }
-int64_t e2k_query_packed_attn_bwd_ws_floats(int nd, int Tq, int H, int max_q, int reach) {
-    if (nd < 0 || Tq < 0 || H < 1 || reach < 0 || reach > REACH_MAX) return 0;
+int64_t e2k_query_packed_attn_bwd_ws_floats(int nd, int Tq, int Tk, int H, int Hkv, int max_q, int reach, int dtable) {
+    if (nd < 0 || Tq < 0 || Tk < 0 || H < 1 || Hkv < 1 || H % Hkv != 0 || reach < 0 || reach > REACH_MAX) return 0;
+    const int s = splits_for(Tk, H, Hkv, max_q, Tq);
+    const int64_t join = s > 1 ? (int64_t)s * 2 * Tk * Hkv * DH : 0;
+    if (!dtable) return join;
     if (max_q <= 0 || max_q > Tq) max_q = Tq;
     const int64_t nt = max_q > 0 ? (max_q + 127) / 128 : 1;
-    return ((Tq > 0 ? nd * nt * H : 0) + H) * (2 * (int64_t)reach + 1);
+    const int64_t sums = ((Tq > 0 ? nd * nt * H : 0) + H) * (2 * (int64_t)reach + 1);
+    return (sums + 3) / 4 * 4 + join;
 }
 int e2k_packed_attn_bwd(const void* dO, int64_t sg, int64_t hg, const void* Q, int64_t sq, int64_t hq, const void* K, int64_t sk, int64_t hk,
                         const void* V, int64_t sv, int64_t hv, const int32_t* cu_q, const int32_t* cu_k, const int32_t* len_q, const int32_t* len_k,

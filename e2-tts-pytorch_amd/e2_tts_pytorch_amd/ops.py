@@ -1171,7 +1171,7 @@ def packed_attn_bwd(st, dout, dtable=None):
     if dout.shape != q.shape or dout.device != dev:
         raise E2KError(f'packed attention: dout must match the output {tuple(q.shape)}, got {tuple(dout.shape)}')
     nd = st.cu_q.numel() - 1
-    ws, acc = None, 0
+    acc = 0
     if st.lo is None:
         if dtable is not None:
             raise E2KError('packed attention: dtable given, but the forward had no table or table_grad=False')
@@ -1182,7 +1182,8 @@ def packed_attn_bwd(st, dout, dtable=None):
             raise E2KError('packed attention: dtable must be contiguous fp32 like the table')
         else:
             acc = 1
-        ws = torch.empty(_lib.get().e2k_query_packed_attn_bwd_ws_floats(nd, Tq, H, st.max_q, st.reach), dtype=f32, device=dev)
+    n = _lib.get().e2k_query_packed_attn_bwd_ws_floats(nd, Tq, Tk, H, Hkv, st.max_q, st.reach, int(dtable is not None))
+    ws = torch.empty(n, dtype=f32, device=dev) if n else None
     dq = torch.empty((Tq, H, 64), dtype=bf16, device=dev)
     dk, dv = (torch.empty((Tk, Hkv, 64), dtype=bf16, device=dev) for _ in range(2))
     delta = torch.empty((H, Tq), dtype=f32, device=dev)

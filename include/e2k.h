@@ -364,8 +364,9 @@ int e2k_packed_attn_fwd(const void* Q, int64_t sq, int64_t hq, const void* K, in
                         const float* table, const int32_t* buckets, int nbuckets, int reach, void* O, int64_t so, int64_t ho, void* Olo,
                         float* lse2, int fill_gaps, void* stream);
 /* dQ (Tq, H, 64), dK, dV (Tk, Hkv, 64) contiguous (uncovered rows as above); delta (H, Tq) scratch.  dtable (may be NULL): gradient of the table,
- * (nbuckets, H) fp32, added to with accumulate = 1; Olo and ws (e2k_query_packed_attn_bwd_ws_floats floats) with dtable, else NULL.  Deterministic. */
-int64_t e2k_query_packed_attn_bwd_ws_floats(int nd, int Tq, int H, int max_q, int reach);
+ * (nbuckets, H) fp32, added to with accumulate = 1; needs Olo.
+ * ws: e2k_query_packed_attn_bwd_ws_floats floats, 16-byte aligned (0: NULL will do).  Deterministic. */
+int64_t e2k_query_packed_attn_bwd_ws_floats(int nd, int Tq, int Tk, int H, int Hkv, int max_q, int reach, int dtable);
 int e2k_packed_attn_bwd(const void* dO, int64_t sg, int64_t hg, const void* Q, int64_t sq, int64_t hq, const void* K, int64_t sk, int64_t hk,
                         const void* V, int64_t sv, int64_t hv, const int32_t* cu_q, const int32_t* cu_k, const int32_t* len_q,
                         const int32_t* len_k, const int32_t* prefix, int nd, int Tq, int Tk, int H, int Hkv, int max_q, int max_k, int causal,

@@ -490,3 +490,16 @@ def test_attn_decode_large(lens, n, kw):
     out = decode(c, lens, n, 'cuda')
     held(out, want, bound, 'out')
     assert torch.equal(out, decode(c, lens, n, 'cuda'))
+
+
+@pytest.mark.parametrize('bias', BIASES)
+@pytest.mark.parametrize('mask', ['full', 'causal'])
+def test_packed_attention_split_sweep(dev, mask, bias):
+    """few key heads, long sweeps: dK / dV in parts (the borders of the parts lie inside a head's tiles), gaps between the documents left zero"""
+    from e2_tts_pytorch_amd import _lib
+    c = Case([600, 100], kl=[70, 100], H=3 if dev == 'cpu' else 6, Hkv=1, nq=[513, 100], nk=[65, 100], mask=mask, bias=bias, tail=4)
+    assert _lib.get().e2k_query_packed_attn_bwd_ws_floats(2, c.q.shape[0], c.k.shape[0], c.H, 1, 600, 0, 0) > 0
+    got = check(c, dev, max_q=600)
+    assert (got['dk'][65:70] == 0).all() and (got['dv'][170:] == 0).all()
+    again = run(c, dev, max_q=600)
+    assert all(torch.equal(got[n], again[n]) for n in got)
