@@ -21,10 +21,10 @@
 // Softmax: the reference point of a row is the maximum of the first block it sees, and stays: fp32 sums and bf16 probabilities lose nothing by a
 // common factor, so nothing is compared per score.  Only when a row's sum passes 2^60 (or overflows: the first block of a row does) is the block's
 // maximum taken, the accumulators rescaled and the block's probabilities taken again -- one compare and a vote per 32-key block.
-// The table's gradient is a sum of the small differences p (dO.v - dO.o) over every pair at a distance, returned in fp32: an o that is good to
-// bf16 only (probabilities rounded before the second product, output rounded after it) would show in its third digit.  A training forward with
-// a table therefore carries the probabilities as two bf16 terms through the second product and keeps what rounding cut off the output (o_lo):
-// dO.o is then good to 2^-16 of its terms.
+// The backward works with small differences p (dO.v - dO.o), and the table's gradient is a sum of them over every pair at a distance, in fp32: an
+// o that is good to bf16 only (probabilities rounded before the second product, output rounded after it) shows in the gradients of q and k (2.9e-3
+// off the exact ones instead of 2.4e-3) and in the third digit of the table's.  A training forward therefore carries the probabilities as two bf16
+// terms through the second product and keeps what rounding cut off the output (o_lo): dO.o is then good to 2^-16 of its terms.
 //
 // Sums are taken in a fixed order throughout: no atomics, the same bits every time.
 #include "e2k_device.h"
@@ -206,8 +206,8 @@ struct Stager {
 
 // One workgroup = 128 queries of one (document, head): 4 waves x 32; K / V tiles of 64 keys through a 2-stage LDS-DMA ring (the next tile in
 // flight while this one is computed, one raw barrier a tile).
-// TR: 0 inference, 1 training (log-sum-exps), 2 training with the table's gradient to come (two-term probabilities, o_lo)
-template <int BIAS, bool CAP, int TR>
+// TRAIN: log-sum-exps, two-term probabilities, o_lo
+template <int BIAS, bool CAP, bool TRAIN>
 __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
     __shared__ __attribute__((aligned(16))) unsigned char smem[NST * STAGE];
     __shared__ float lut[BIAS == 2 ? 2 * REACH_MAX + 1 + 2 * PADL : 1];
@@ -222,7 +222,8 @@ __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
     const int h = wk.h;
     const Doc D = doc_of(p, wk.d);
     if (wk.tile * 128 >= D.nq) return;
-    Scorer<BIAS, CAP, 1, TR == 2, false> sc;
+    constexpr bool FINE = TRAIN && BIAS == 2;          // (the table's gradient is returned in fp32)
+    Scorer<BIAS, CAP, 1, FINE, false> sc;
     sc.init(p, BIAS == 1 ? p.slopes[h] : 0.f);
     if (BIAS == 2) {
         load_lut(p, h, lut);
@@ -259,7 +260,8 @@ __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
         if (nt > 0) fetch(0, smem);
         if (nt > 1) fetch(1, smem + STAGE);
         const int qp = q0 + D.off;
-        // probabilities (arguments of exp2 in x) packed, the row's sum with them (training with a table: fp32 sums and a second term)
+        // probabilities (arguments of exp2 in x) packed, in training with what packing cut off as a second term, and the row's sum with them (of the
+        // packed ones: its error is theirs over the square root of their number; of the unrounded ones where fp32 results depend on it)
         auto probs = [&](float (&x)[16], bf16x8 (&pf)[2], bf16x8 (&pl)[2], float& la, float& lb) __attribute__((always_inline)) {
             la = l0;
             lb = l1;
@@ -267,12 +269,20 @@ __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
             for (int r = 0; r < 16; ++r) x[r] = fast_exp2(x[r]);
             pf[0] = pack8f(x);
             pf[1] = pack8f(x + 8);
-            if (TR == 2) {
+            if (FINE) {
 #pragma unroll
                 for (int r = 0; r < 16; r += 2) {
                     la += x[r];
                     lb += x[r + 1];
                 }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    la = add_bf16_pair(__builtin_bit_cast(u32x4, pf[0])[i], la);
+                    lb = add_bf16_pair(__builtin_bit_cast(u32x4, pf[1])[i], lb);
+                }
+            }
+            if (TRAIN) {
 #pragma unroll
                 for (int s2 = 0; s2 < 2; ++s2) {
                     float w[8];
@@ -280,12 +290,6 @@ __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) w[e] = x[8 * s2 + e] - w[e];
                     pl[s2] = pack8f(w);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    la = add_bf16_pair(__builtin_bit_cast(u32x4, pf[0])[i], la);
-                    lb = add_bf16_pair(__builtin_bit_cast(u32x4, pf[1])[i], lb);
                 }
             }
         };
@@ -351,7 +355,7 @@ __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
                 for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
                     for (int db = 0; db < 2; ++db) o[db] = mfma32(vf[s2][db], pf[s2], o[db]);
-                if (TR == 2) {
+                if (TRAIN) {
 #pragma unroll
                     for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
@@ -371,15 +375,15 @@ __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
             l += lane32_other(l);                             // a row's keys are split over lanes l and l + 32
             const float inv = l == 0.f ? 0.f : 1.f / l;       // (NaN stays NaN)
             const int row = D.q0 + (qin ? q : 0);
-            if (TR && qin && hi == 0) p.lse2[(long)h * p.Tq + row] = l == 0.f ? LSE_EMPTY : m + log2f(l);
+            if (TRAIN && qin && hi == 0) p.lse2[(long)h * p.Tq + row] = l == 0.f ? LSE_EMPTY : m + log2f(l);
             bf16_t* orow = p.O + (long)row * p.so + (long)h * p.ho;
-            bf16_t* lrow = TR == 2 ? p.Olo + ((long)row * p.H + h) * DH : nullptr;
+            bf16_t* lrow = TRAIN ? p.Olo + ((long)row * p.H + h) * DH : nullptr;
             store_rows32(o, hi, qin, [&](int db, int g, int hi_, bool ok, const float* a, const float* b) __attribute__((always_inline)) {
                 float v[8];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) { v[e] = a[e] * inv; v[4 + e] = b[e] * inv; }
                 u32x2 x = pack4(v), y = pack4(v + 4), xl, yl;
-                if (TR == 2) {
+                if (TRAIN) {
                     float w[8], lo[8];
                     unpack4(x, w);
                     unpack4(y, w + 4);
@@ -393,7 +397,7 @@ __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
                 const int col = 32 * db + 8 * (g + hi_);
                 if (ok) {
                     st<u32x4>(orow + col, u32x4{x[0], x[1], y[0], y[1]});
-                    if (TR == 2) st<u32x4>(lrow + col, u32x4{xl[0], xl[1], yl[0], yl[1]});
+                    if (TRAIN) st<u32x4>(lrow + col, u32x4{xl[0], xl[1], yl[0], yl[1]});
                 }
             });
         }
@@ -492,10 +496,10 @@ __global__ __launch_bounds__(256, (BIAS || CAP) ? 2 : 3) void pa_dq_kernel(PAArg
             for (int ks = 0; ks < 4; ++ks) {
                 float a[8], b[8], g[8];
                 unpack8(ld<u32x4>(orow + ks * 16), a);
-                if (RG) unpack8(ld<u32x4>(lrow + ks * 16), b);
+                unpack8(ld<u32x4>(lrow + ks * 16), b);
                 unpack8(__builtin_bit_cast(u32x4, dof[ks]), g);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) dl = fmaf(g[e], RG ? a[e] + b[e] : a[e], dl);
+                for (int e = 0; e < 8; ++e) dl = fmaf(g[e], a[e] + b[e], dl);
             }
             dl += lane32_other(dl);
             if (qin && hi == 0) p.delta[(long)h * p.Tq + row] = dl;
@@ -898,10 +902,9 @@ int plan_grid(PAArgs& a, int longest, int total, int heads, long& grid) {
     return E2K_OK;
 }
 
-template <int BIAS, bool CAP> void run_fwd(const PAArgs& a, int train, long grid, hipStream_t st) {
-    if (BIAS == 2 && train == 2) hipLaunchKernelGGL((pa_fwd_kernel<BIAS, CAP, BIAS == 2 ? 2 : 1>), dim3((unsigned)grid), dim3(256), 0, st, a);
-    else if (train) hipLaunchKernelGGL((pa_fwd_kernel<BIAS, CAP, 1>), dim3((unsigned)grid), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((pa_fwd_kernel<BIAS, CAP, 0>), dim3((unsigned)grid), dim3(256), 0, st, a);
+template <int BIAS, bool CAP> void run_fwd(const PAArgs& a, bool train, long grid, hipStream_t st) {
+    if (train) hipLaunchKernelGGL((pa_fwd_kernel<BIAS, CAP, true>), dim3((unsigned)grid), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((pa_fwd_kernel<BIAS, CAP, false>), dim3((unsigned)grid), dim3(256), 0, st, a);
 }
 template <int BIAS, bool CAP> void run_dq(const PAArgs& a, int rg, long grid, hipStream_t st) {
     if (BIAS == 2 && rg == 1) hipLaunchKernelGGL((pa_dq_kernel<BIAS, CAP, BIAS == 2 ? 128 : 0>), dim3((unsigned)grid), dim3(256), 0, st, a);
@@ -943,14 +946,14 @@ int packed_attn_fwd_impl(const void* Q, int64_t sq, int64_t hq, const void* K, i
     if (Tq == 0) return E2K_OK;
     const int rc = check(a);
     if (rc) return rc;
-    if (!O || (Olo && (!lse2 || !table))) return E2K_ERR_ARG;
+    if (!O || (!Olo) != (!lse2)) return E2K_ERR_ARG;
     if (!aligned16(Olo)) return E2K_ERR_ALIGN;
     long grid;
     const int rg = plan_grid(a, max_q, Tq, H, grid);
     if (rg) return rg;
     if (grid == 0) return E2K_OK;
     hipStream_t st = (hipStream_t)stream;
-    PA_PICK(run_fwd, a, Olo ? 2 : lse2 ? 1 : 0, grid, st);
+    PA_PICK(run_fwd, a, Olo != nullptr, grid, st);
     E2K_CHECK_LAUNCH();
     return E2K_OK;
 }
@@ -970,7 +973,7 @@ int packed_attn_bwd_impl(const void* dO, int64_t sg, int64_t hg, const void* Q, 
     if (Tq > 0) {
         const int rc = check(a);
         if (rc) return rc;
-        if (!dO || !O || !lse2 || !delta || !dQ || (dtable && (!table || !ws || !Olo))) return E2K_ERR_ARG;
+        if (!dO || !O || !Olo || !lse2 || !delta || !dQ || (dtable && (!table || !ws))) return E2K_ERR_ARG;
         if (!strides_ok(sg, hg) || !aligned16(dO) || !aligned16(Olo) || !aligned16(dQ) || !aligned16(dK) || !aligned16(dV)) return E2K_ERR_ALIGN;
         if (Tk > 0 && (!dK || !dV)) return E2K_ERR_ARG;
         const int rg = plan_grid(a, max_q, Tq, H, grid);

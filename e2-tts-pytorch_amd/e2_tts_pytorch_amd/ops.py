@@ -1105,13 +1105,13 @@ class PackedAttnState:
 
 
 def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, len_q=None, len_k=None, prefix=None, max_q=0, max_k=0, causal=False, scale=None, softcap=0., slopes=None,
-                    table=None, buckets=None, out=None, train=False, table_grad=True):
+                    table=None, buckets=None, out=None, train=False):
     """Attention over documents that lie one behind the other: q (Tq,H,64), k / v (Tk,Hkv,64) bf16 with Hkv dividing H; document d has the query rows
     cu_q[d]:cu_q[d+1] and the key rows cu_k[d]:cu_k[d+1] (int32 offsets on the device; cu_k None: the same as cu_q), only the first len_q[d] /
     len_k[d] of them where given (int32).  causal: a query sees the keys up to its own position (the last query stands on the last key) and the first
     prefix[d] keys.  softcap > 0: scores capped to softcap * tanh(score / softcap).  slopes (H,) fp32: bias -slope * distance; or table (buckets,H) fp32
     with buckets (2 reach + 1,) int32: learned bias by key - query distance (rel_buckets).  max_q / max_k: longest document, a sizing hint.
-    -> out (Tq,H,64) bf16, with train=True (out, state for packed_attn_bwd; table_grad=False: without the table's gradient).  Rows that no document covers: zero, or left alone in an `out` given by the
+    -> out (Tq,H,64) bf16, with train=True (out, state for packed_attn_bwd).  Rows that no document covers: zero, or left alone in an `out` given by the
     caller.  Offsets have to be non-decreasing.  NaN / inf outside a document never reaches it; inside, a NaN / inf key or value may reach any query of
     its document.  Biases of -1e30 or less hide their keys."""
     _chk(q, k, v, cu_q, cu_k, len_q, len_k, prefix, slopes, table, buckets, out)
@@ -1144,7 +1144,7 @@ def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, len_q=None, len_k=None, prefix=
         raise E2KError('packed attention: out must be a (Tq, H, 64) bf16 tensor like q with 16-byte rows that do not overlap')
     lo = lse2 = None
     if train:
-        lo = torch.empty((Tq, H, 64), dtype=bf16, device=dev) if table is not None and table_grad else None
+        lo = torch.empty((Tq, H, 64), dtype=bf16, device=dev)
         lse2 = torch.empty((H, Tq), dtype=f32, device=dev)
     with _on_device(q):
         _lib.get().e2k_packed_attn_fwd(_p(q), q.stride(0), q.stride(1), _p(k), k.stride(0), k.stride(1), _p(v), v.stride(0), v.stride(1), _p(cu_q), _p(cu_k),
@@ -1159,9 +1159,9 @@ def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, len_q=None, len_k=None, prefix=
     return out, st
 
 
-def packed_attn_bwd(st, dout, dtable=None):
+def packed_attn_bwd(st, dout, dtable=None, need_table=True):
     """-> (dq, dk, dv, dtable): gradients of packed_attn_fwd(train=True), contiguous bf16 (rows that no document covers are zero); dtable fp32 (buckets,H) is
-    ADDED TO where given, fresh where not, None without a table or after a forward with table_grad=False"""
+    ADDED TO where given, fresh where not, None without a table or with need_table=False"""
     _chk(dout, dtable)
     q, k, v = st.q, st.k, st.v
     dout = _heads64(dout, 'dout')
@@ -1172,9 +1172,9 @@ def packed_attn_bwd(st, dout, dtable=None):
         raise E2KError(f'packed attention: dout must match the output {tuple(q.shape)}, got {tuple(dout.shape)}')
     nd = st.cu_q.numel() - 1
     acc = 0
-    if st.lo is None:
+    if st.table is None or not need_table:
         if dtable is not None:
-            raise E2KError('packed attention: dtable given, but the forward had no table or table_grad=False')
+            raise E2KError('packed attention: dtable given without a table, or with need_table=False')
     else:
         if dtable is None:
             dtable = torch.empty_like(st.table)

@@ -20,7 +20,7 @@ class _PackedAttnFn(Function):
         train = any(ctx.needs_input_grad[:4])
         if not train:
             return ops.packed_attn_fwd(q, k, v, cu_q, cu_k, table=table, **kw)
-        out, st = ops.packed_attn_fwd(q, k, v, cu_q, cu_k, table=table, train=True, table_grad=ctx.needs_input_grad[3], **kw)
+        out, st = ops.packed_attn_fwd(q, k, v, cu_q, cu_k, table=table, train=True, **kw)
         # tensors autograd has to watch (an input or the output changed in place before the backward raises) go through save_for_backward
         ctx.save_for_backward(q, k, v, table, out, kw['slopes'], kw['buckets'], cu_q, cu_k, kw['len_q'], kw['len_k'], kw['prefix'])
         st.out = None
@@ -36,8 +36,8 @@ class _PackedAttnFn(Function):
         for name in ops.PackedAttnState.__slots__:
             setattr(full, name, getattr(st, name))
         full.out = saved[4]
-        dq, dk, dv, dtable = ops.packed_attn_bwd(full, dout)
         need = ctx.needs_input_grad
+        dq, dk, dv, dtable = ops.packed_attn_bwd(full, dout, need_table=need[3])
         return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dtable if need[3] else None, None, None, None
 
 
