@@ -32,7 +32,9 @@ struct DecodeArgs {
     bf16_t* O; float* ws;
 };
 
-template <int BIAS, bool CAP>
+// HEADS: the four waves of a workgroup take the same keys of four neighbouring key heads (512 consecutive bytes of every cache row), else four
+// runs of keys of one head, joined here.
+template <int BIAS, bool CAP, bool HEADS>
 __global__ __launch_bounds__(NW * 64, 2) void attn_decode_kernel(DecodeArgs p) {
     __shared__ __attribute__((aligned(16))) unsigned char smem[NW * STAGES * BLK];
     __shared__ float ml[NW][2][32];
@@ -41,13 +43,14 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_decode_kernel(DecodeArgs p) {
     const int l31 = lane & 31, hi = lane >> 5;
     // key heads fastest: neighbouring workgroups read neighbouring parts of the same rows
     int lin = (int)blockIdx.x;
-    const int hk = lin % p.Hkv; lin /= p.Hkv;
-    const int grp = lin % p.ngrp; lin /= p.ngrp;
+    const int nhk = HEADS ? p.Hkv / NW : p.Hkv;
+    const int hk = HEADS ? lin % nhk * NW + wave : lin % nhk; lin /= nhk;
+    const int grp = HEADS ? 0 : lin % p.ngrp; lin /= p.ngrp;
     const int split = lin % p.splits, b = lin / p.splits;
     const int cols = min(32, p.G - 32 * grp), h0 = hk * p.G + 32 * grp;        // query heads h0 .. h0 + cols - 1
     const int n = uniform_i(clampi(p.lens[b], 0, p.cap_n));
     const int nblk = (n + 31) / 32;                                            // 32-key blocks of the sequence, shared evenly by splits x waves
-    const long parts = (long)p.splits * NW, me = (long)split * NW + wave;
+    const long parts = HEADS ? p.splits : (long)p.splits * NW, me = HEADS ? split : (long)split * NW + wave;
     const int b0 = (int)(nblk * me / parts), b1 = (int)(nblk * (me + 1) / parts);
 
     const bool col = l31 < cols;
@@ -190,64 +193,78 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_decode_kernel(DecodeArgs p) {
         if (hi == 0) { ml[wave][0][l31] = m; ml[wave][1][l31] = l; }
     }
     __syncthreads();
-    for (int i = tid; i < cols * DH; i += NW * 64) {
-        const int cc = i / DH, d = i % DH;
-        float M = ml[0][0][cc], L = 0.f, a = 0.f;
+    for (int i = tid; i < (HEADS ? NW : 1) * cols * DH; i += NW * 64) {
+        const int cc = i / DH % cols, d = i % DH, w0 = HEADS ? i / DH / cols : 0;
+        const int hh = HEADS ? (hk - wave + w0) * p.G + cc : h0 + cc;
+        float M = ml[w0][0][cc], L = 0.f, a = 0.f;
+        if (!HEADS) {
 #pragma unroll
-        for (int w = 1; w < NW; ++w) M = fmaxf(M, ml[w][0][cc]);
+            for (int w = 1; w < NW; ++w) M = fmaxf(M, ml[w][0][cc]);
+        }
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            const float e = fast_exp2(ml[w][0][cc] - M);
-            L = fmaf(ml[w][1][cc], e, L);
-            a = fmaf(acc[(w * cols + cc) * DH + d], e, a);
+        for (int w = 0; w < (HEADS ? 1 : NW); ++w) {
+            const float e = HEADS ? 1.f : fast_exp2(ml[w][0][cc] - M);
+            L = fmaf(ml[w0 + w][1][cc], e, L);
+            a = fmaf(acc[((w0 + w) * cols + cc) * DH + d], e, a);
         }
         if (p.splits == 1) {
-            p.O[(long)b * p.ob + (long)(h0 + cc) * p.oh + d] = f2bf(L == 0.f ? 0.f : a / L);
+            p.O[(long)b * p.ob + (long)hh * p.oh + d] = f2bf(L == 0.f ? 0.f : a / L);
         } else {
-            float* q = p.ws + (((long)b * p.H + h0 + cc) * p.splits + split) * PART;
+            float* q = p.ws + (((long)b * p.H + hh) * p.splits + split) * PART;
             q[d] = a;
             if (d == 0) { q[DH] = M; q[DH + 1] = L; }
         }
     }
 }
 
-// one wave per (sequence, query head): lane = output column
+// one workgroup per (sequence, query head): lane = output column, the waves take a quarter of the parts each
 __global__ __launch_bounds__(256) void attn_decode_join_kernel(DecodeArgs p) {
-    const int lane = threadIdx.x & 63;
-    const long w = (long)blockIdx.x * 4 + uniform_i(threadIdx.x >> 6);
-    if (w >= (long)p.B * p.H) return;
+    __shared__ float sm[4][DH], sl[4];
+    const int lane = threadIdx.x & 63, wave = uniform_i(threadIdx.x >> 6);
+    const long w = blockIdx.x;
     const float* q = p.ws + w * p.splits * PART;
     float M = M_INIT;
     for (int s = lane; s < p.splits; s += 64) M = fmaxf(M, q[(long)s * PART + DH]);
     M = wave_max(M);
     float L = 0.f, a = 0.f;
 #pragma unroll 8
-    for (int s = 0; s < p.splits; ++s) {
+    for (int s = wave; s < p.splits; s += 4) {
         const float* r = q + (long)s * PART;
         const float e = fast_exp2(r[DH] - M);
         L = fmaf(r[DH + 1], e, L);
         a = fmaf(r[lane], e, a);
     }
-    p.O[(w / p.H) * p.ob + (w % p.H) * p.oh + lane] = f2bf(L == 0.f ? 0.f : a / L);
+    sm[wave][lane] = a;
+    if (lane == 0) sl[wave] = L;
+    __syncthreads();
+    if (wave == 0) {
+        a = (sm[0][lane] + sm[1][lane]) + (sm[2][lane] + sm[3][lane]);
+        L = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+        p.O[(w / p.H) * p.ob + (w % p.H) * p.oh + lane] = f2bf(L == 0.f ? 0.f : a / L);
+    }
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 bool ok8(long s) { return s >= 0 && s % 8 == 0; }
 
-// Workgroups per (sequence, key head): about 1024 keys each (eight blocks a wave: the start of a wave is a few blocks' time), fewer keys where that
-// leaves the chip's 512 workgroup slots empty, never less than one block a wave; at most 128
+// The four waves of a workgroup read four key heads' rows side by side where the heads come in fours (and a pass has all query heads of one)
+bool by_heads(int Hkv, int G) { return Hkv % NW == 0 && G <= 32; }
+// Parts of a sequence's keys: about 256 keys a wave (eight blocks: the start of a wave is a few blocks' time), fewer where that leaves the chip's
+// 512 workgroup slots empty, never less than one block a wave; at most 128 (the join reads them all)
 int splits_for(int B, int cap_n, int Hkv, int G) {
-    const long pairs = (long)B * Hkv * ((G + 31) / 32);
-    long s = (cap_n + 512) / 1024;
-    if (pairs * s < 512) s = (512 + pairs - 1) / pairs;
-    const long most = (cap_n + NW * 32 - 1) / (NW * 32);
+    const int run = by_heads(Hkv, G) ? 1 : NW;                      // waves that share a part
+    const long wgs = (long)B * (by_heads(Hkv, G) ? Hkv / NW : (long)Hkv * ((G + 31) / 32));
+    long s = (cap_n + 128 * run) / (256 * run);
+    if (wgs * s < 512) s = (512 + wgs - 1) / wgs;
+    const long most = (cap_n + run * 32 - 1) / (run * 32);
     if (s > most) s = most;
     if (s > 128) s = 128;
     return (int)(s < 1 ? 1 : s);
 }
 
 template <int BIAS, bool CAP> void run(const DecodeArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL((attn_decode_kernel<BIAS, CAP>), dim3((unsigned)((long)a.B * a.splits * a.ngrp * a.Hkv)), dim3(NW * 64), 0, st, a);
+    if (by_heads(a.Hkv, a.G)) hipLaunchKernelGGL((attn_decode_kernel<BIAS, CAP, true>), dim3((unsigned)((long)a.B * a.splits * (a.Hkv / NW))), dim3(NW * 64), 0, st, a);
+    else hipLaunchKernelGGL((attn_decode_kernel<BIAS, CAP, false>), dim3((unsigned)((long)a.B * a.splits * a.ngrp * a.Hkv)), dim3(NW * 64), 0, st, a);
 }
 
 int attn_decode_impl(const void* Q, int64_t qb, int64_t qh, const void* K, int64_t kb, int64_t kn, int64_t kh, const void* V, int64_t vb, int64_t vn,
@@ -269,7 +286,7 @@ int attn_decode_impl(const void* Q, int64_t qb, int64_t qh, const void* K, int64
     a.scale = scale; a.cap = softcap; a.slopes = slopes; a.table = table; a.buckets = buckets; a.nbuckets = nbuckets; a.R = reach;
     a.O = (bf16_t*)O; a.ws = ws;
     if (a.splits > 1 && !ws) return E2K_ERR_ARG;
-    if ((long)B * a.splits * a.ngrp * Hkv > 0x7fffffffL / (NW * 64)) return E2K_ERR_SHAPE;
+    if ((long)B * a.splits * a.ngrp * Hkv > 0x7fffffffL / (NW * 64) || (long)B * H > 0x7fffffffL / 256) return E2K_ERR_SHAPE;
     hipStream_t st = (hipStream_t)stream;
     const bool c = softcap > 0.f;
     if (table) { if (c) run<2, true>(a, st); else run<2, false>(a, st); }
@@ -277,7 +294,7 @@ int attn_decode_impl(const void* Q, int64_t qb, int64_t qh, const void* K, int64
     else { if (c) run<0, true>(a, st); else run<0, false>(a, st); }
     E2K_CHECK_LAUNCH();
     if (a.splits > 1) {
-        hipLaunchKernelGGL(attn_decode_join_kernel, dim3((unsigned)(((long)B * H + 3) / 4)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL(attn_decode_join_kernel, dim3((unsigned)((long)B * H)), dim3(256), 0, st, a);
         E2K_CHECK_LAUNCH();
     }
     return E2K_OK;

@@ -5,7 +5,7 @@
 //
 // What bounds it: HBM (x and y once; x, dy and dx once).  A row stays in registers between its two reductions (mean first, then the
 // centred squares: no cancellation however far the mean lies from 0); the next row of the wave is loaded while the current one is
-// reduced.  64 lanes own a row up to 2048 columns, 256 lanes beyond (up to 8192).  Rows whose addresses or width are not multiples of
+// reduced.  64 lanes own a row up to 1536 columns, 256 lanes beyond (up to 8192).  Rows whose addresses or width are not multiples of
 // 16 bytes take element-wise accesses (still whole lines per wave instruction).
 // The sums over rows of the backward stay in registers over all rows of a wave, are joined in LDS in a fixed order, and leave as one
 // partial row per workgroup; a second kernel adds the partials in a fixed order: no atomics, the same bits every time.
@@ -20,6 +20,7 @@ namespace {
 
 constexpr int LN_MAX = 8192;            // widest row (256 lanes x 32 elements)
 constexpr int LN_WAVES = 8;             // waves per workgroup of the backward
+constexpr int LN_ROW64 = 1536;          // widest row of 64 lanes: 24 elements a lane (32 of them and the backward's sums do not fit a wave's registers)
 
 struct LNArgs {
     const void* x; long ldx;
@@ -73,16 +74,27 @@ __device__ __forceinline__ void store_elems(T* row, int t, int D, const float (&
         }
     }
 }
-// per-column fp32 vector (gamma / beta); `none` where there is none
+// per-column fp32 vector (gamma / beta), 16 bytes at a time where the rows are; `none` where there is none
 template <int VEC, int NCH, int LPR>
 __device__ __forceinline__ void load_cols(const float* p, float off, float none, int t, int D, float (&v)[VEC * NCH]) {
 #pragma unroll
-    for (int c = 0; c < NCH; ++c)
+    for (int e = 0; e < VEC * NCH; ++e) v[e] = none;
+    if (!p) return;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const int col = (c * LPR + t) * VEC + i;
-            v[c * VEC + i] = (p && col < D) ? p[col] + off : none;
+    for (int c = 0; c < NCH; ++c) {
+        const int col = (c * LPR + t) * VEC;
+        if (col >= D) continue;
+        if (VEC == 1) {
+            v[c] = p[col] + off;
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; i += 4) {
+                const f32x4 w = ld<f32x4>(p + col + i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[c * VEC + i + j] = w[j] + off;
+            }
         }
+    }
 }
 
 // sums over the LPR lanes of a row; with 256 lanes every wave of the workgroup takes part (buf: 2 floats per wave, double-buffered by `ph`)
@@ -116,7 +128,7 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(LNArgs p, int share) {
         if (r >= p.M) break;           // (uniform over the lanes that meet in a reduction: a wave, or the workgroup that is one row slot)
         const Row<T, VEC, NCH, LPR> x = nx;
         if (s + 1 < share && r + RPW < p.M) nx.load((const T*)p.x + (r + RPW) * p.ldx, t, p.D);
-        const int bi = (int)(r / p.rpb);
+        const int bi = (int)((unsigned)r / (unsigned)p.rpb);
         if (bi != cur) {
             cur = bi;
             load_cols<VEC, NCH, LPR>(p.gamma ? p.gamma + bi * p.ldg : nullptr, p.gamma_off, 1.f, t, p.D, w);
@@ -276,21 +288,22 @@ template <class T, int VEC, int NCH, int LPR> int launch_bwd(const LNArgs& a, hi
     do {                                                                                          \
         constexpr int V_ = VEC;                                                                   \
         const int per = (a.D + V_ - 1) / V_;                                                      \
-        if (a.D <= 64 * 32) {                                                                     \
+        if (a.D <= LN_ROW64) {                                                                    \
             const int ch = (per + 63) / 64;                                                       \
             if (ch <= 8 / V_) return FN<T, V_, 8 / V_, 64>(a, st);                                \
             if (ch <= 16 / V_) return FN<T, V_, 16 / V_, 64>(a, st);                              \
-            if (ch <= 24 / V_) return FN<T, V_, 24 / V_, 64>(a, st);                              \
-            return FN<T, V_, 32 / V_, 64>(a, st);                                                 \
+            return FN<T, V_, 24 / V_, 64>(a, st);                                                 \
         }                                                                                         \
         const int ch = (per + 255) / 256;                                                         \
+        if (ch <= 8 / V_) return FN<T, V_, 8 / V_, 256>(a, st);                                   \
         if (ch <= 16 / V_) return FN<T, V_, 16 / V_, 256>(a, st);                                 \
         return FN<T, V_, 32 / V_, 256>(a, st);                                                    \
     } while (0)
 
-// workgroups per batch element of the backward: about one workgroup (eight waves) per CU over all batch elements
+// workgroups per batch element of the backward: at most one (eight waves) per CU over all batch elements -- a 257th workgroup would share a CU and
+// finish at half the speed of the others (16399 rows of 1003: 34 us with 256, 44 with 257)
 int bwd_gpb(int M, int D, int rpb) {
-    const int nb = (M + rpb - 1) / rpb, slots = D <= 2048 ? LN_WAVES : LN_WAVES / 4;
+    const int nb = (M + rpb - 1) / rpb, slots = D <= LN_ROW64 ? LN_WAVES : LN_WAVES / 4;
     const int most = (rpb + slots - 1) / slots;
     int g = 256 / nb;
     if (g > most) g = most;
@@ -316,7 +329,8 @@ int layernorm_fwd_impl(const void* x, int64_t ldx, int dtype, const float* gamma
     a.M = M; a.D = D; a.rpb = rows_per_batch; a.nb = (M + rows_per_batch - 1) / rows_per_batch; a.eps = eps;
     hipStream_t st = (hipStream_t)stream;
     const int vec = dtype == 0 ? 8 : 4;
-    const bool wide = D % vec == 0 && ldx % vec == 0 && aligned16(x) && aligned16(y);
+    const bool cols = aligned16(gamma) && aligned16(beta) && (ldg % 4 == 0 || M <= rows_per_batch);
+    const bool wide = cols && D % vec == 0 && ldx % vec == 0 && aligned16(x) && aligned16(y);
     if (dtype == 0) {
         if (wide) LN_PICK(launch_fwd, bf16_t, 8);
         LN_PICK(launch_fwd, bf16_t, 1);
@@ -339,7 +353,8 @@ int layernorm_bwd_impl(const void* dy, const void* x, int64_t ldx, int dtype, co
     a.M = M; a.D = D; a.rpb = rows_per_batch; a.nb = (M + rows_per_batch - 1) / rows_per_batch; a.gpb = bwd_gpb(M, D, rows_per_batch);
     hipStream_t st = (hipStream_t)stream;
     const int vec = dtype == 0 ? 8 : 4;
-    const bool wide = D % vec == 0 && ldx % vec == 0 && aligned16(x) && aligned16(dy) && aligned16(dx);
+    const bool cols = aligned16(gamma) && (ldg % 4 == 0 || M <= rows_per_batch);
+    const bool wide = cols && D % vec == 0 && ldx % vec == 0 && aligned16(x) && aligned16(dy) && aligned16(dx);
     const int rl = [&]() -> int {
         if (dtype == 0) {
             if (wide) LN_PICK(launch_bwd, bf16_t, 8);
