@@ -58,7 +58,8 @@ struct PAArgs {
     bf16_t *dQ, *dK, *dV;                              // (Tq, H, 64), (Tk, Hkv, 64)
     float* dist;                                       // [workgroup of the dQ grid][2 R + 1]: sums of dS by distance
     int nt, nwork;                                     // row tiles per (document, head) of this grid; workgroups that compute
-    int splits; float* part;                           // dK / dV: parts of a key tile's sweep, their sums [part][dK | dV][Tk][Hkv][64]
+    int splits; float* part;                           // parts of a tile's sweep; dK / dV: their sums [part][dK | dV][Tk][Hkv][64]; forward: their
+                                                       // accumulators [part][Tq][H][64], then reference points and sums [part][2][Tq][H]
 };
 
 // rows of document d, kept inside [0, total) whatever the offsets say
@@ -204,6 +205,8 @@ struct Stager {
 
 // ------------------------------------------------------------------------------------------------ forward
 
+// Few queries over many keys (prompts behind a cache) leave most of the chip empty and are bound by the latency of a block's chain: inference then
+// cuts a row's keys into parts and joins them.
 // One workgroup = 128 queries of one (document, head): 4 waves x 32; K / V tiles of 64 keys through a 2-stage LDS-DMA ring (the next tile in
 // flight while this one is computed, one raw barrier a tile).
 // TRAIN: log-sum-exps, two-term probabilities, o_lo
@@ -219,7 +222,7 @@ __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform_i(tid >> 6);
     const int l31 = lane & 31, hi = lane >> 5;
     const Work wk = work_of(p);
-    const int h = wk.h;
+    const int h = wk.h / p.splits, part = wk.h % p.splits;
     const Doc D = doc_of(p, wk.d);
     if (wk.tile * 128 >= D.nq) return;
     constexpr bool FINE = TRAIN && BIAS == 2;          // (the table's gradient is returned in fp32)
@@ -247,7 +250,8 @@ __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
         const int qc = min(q, D.nq - 1);              // (lanes past the end repeat the last query: their sums stay in step with the wave's)
         const int lim = D.lim(qc);
         const int lim_lo = live ? D.lim(q0) : 0, lim_hi = live ? D.lim(min(q0 + 31, D.nq - 1)) : 0;
-        const int kend = D.lim(min(tile * 128 + 127, D.nq - 1)), nt = (kend + 63) / 64;
+        const int kend = D.lim(min(tile * 128 + 127, D.nq - 1)), all = (kend + 63) / 64;
+        const int kt0 = all * part / p.splits, nt = all * (part + 1) / p.splits;          // this part's key tiles
         bf16x8 qf[4];
         row_frags(qf, p.Q + (long)(D.q0 + qc) * p.sq + (long)h * p.hq, live, hi);
         f32x16 o[2] = {zero16(), zero16()};
@@ -257,8 +261,8 @@ __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
         auto fetch = [&](int kt, unsigned char* S) __attribute__((always_inline)) {
             sg.issue(Kb + (long)(kt * 64) * p.sk, Vb + (long)(kt * 64) * p.sv, D.nk - 1 - kt * 64, S);
         };
-        if (nt > 0) fetch(0, smem);
-        if (nt > 1) fetch(1, smem + STAGE);
+        if (kt0 < nt) fetch(kt0, smem);
+        if (kt0 + 1 < nt) fetch(kt0 + 1, smem + STAGE);
         const int qp = q0 + D.off;
         // probabilities (arguments of exp2 in x) packed, in training with what packing cut off as a second term, and the row's sum with them (of the
         // packed ones: its error is theirs over the square root of their number; of the unrounded ones where fp32 results depend on it)
@@ -365,14 +369,29 @@ __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
             block(Int<0>{});
             block(Int<1>{});
         };
-        for (int kt = 0; kt < nt; kt += NST) {
+        for (int kt = kt0; kt < nt; kt += NST) {
             step(Int<0>{}, kt);
             if (kt + 1 < nt) step(Int<1>{}, kt + 1);
             if (kt + 2 < nt) step(Int<2>{}, kt + 2);
         }
-        if (live) {
-            float l = l0 + l1;
-            l += lane32_other(l);                             // a row's keys are split over lanes l and l + 32
+        float l = l0 + l1;
+        l += lane32_other(l);                                 // a row's keys are split over lanes l and l + 32
+        if (!TRAIN && p.splits > 1) {
+            if (qin) {
+                const long row = (long)part * p.Tq + D.q0 + q;
+                float* ws = p.part + (row * p.H + h) * DH;
+#pragma unroll
+                for (int db = 0; db < 2; ++db)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                        st<f32x4>(ws + 32 * db + 8 * g + 4 * hi, f32x4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]});
+                if (hi == 0) {
+                    float* ml = p.part + (long)p.splits * p.Tq * p.H * DH + ((long)part * 2 * p.Tq + D.q0 + q) * p.H + h;
+                    ml[0] = m;
+                    ml[(long)p.Tq * p.H] = l;
+                }
+            }
+        } else if (live) {
             const float inv = l == 0.f ? 0.f : 1.f / l;       // (NaN stays NaN)
             const int row = D.q0 + (qin ? q : 0);
             if (TRAIN && qin && hi == 0) p.lse2[(long)h * p.Tq + row] = l == 0.f ? LSE_EMPTY : m + log2f(l);
@@ -402,6 +421,38 @@ __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
             });
         }
         if ((tile + p.nt) * 128 < D.nq) __syncthreads();         // (another round: the ring is free again)
+    }
+}
+
+constexpr int JOIN_ROWS = 4;          // rows of a join workgroup: a thread or two per eight columns (with 32 the few workgroups took 43 us for 890 rows)
+// outputs from the parts of their sweeps; eight columns a thread
+__global__ __launch_bounds__(256) void pa_fwd_join_kernel(PAArgs p) {
+    const int tile = (int)blockIdx.x % p.nt, d = (int)blockIdx.x / p.nt;
+    const Span s = span(p.cu_q, p.len_q, d, p.Tq);
+    const float* ml = p.part + (long)p.splits * p.Tq * p.H * DH;
+    const long step = (long)p.Tq * p.H;
+    for (int r0 = tile * JOIN_ROWS; r0 < s.n; r0 += p.nt * JOIN_ROWS) {
+        const int rows = min(JOIN_ROWS, s.n - r0);
+        for (int i = threadIdx.x; i < rows * p.H * (DH / 8); i += 256) {
+            const int c = i & 7, h = (i >> 3) % p.H, row = s.at + r0 + (i >> 3) / p.H;
+            const long at = (long)row * p.H + h;
+            float M = M_INIT, L = 0.f, a[8];
+            for (int q = 0; q < p.splits; ++q) M = fmaxf(M, ml[2 * q * step + at]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) a[e] = 0.f;
+            for (int q = 0; q < p.splits; ++q) {
+                const float w = fast_exp2(ml[2 * q * step + at] - M);
+                const float* x = p.part + (q * step + at) * DH + 8 * c;
+                const f32x4 u = ld<f32x4>(x), v = ld<f32x4>(x + 4);
+                L = fmaf(ml[(2 * q + 1) * step + at], w, L);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { a[e] = fmaf(u[e], w, a[e]); a[4 + e] = fmaf(v[e], w, a[4 + e]); }
+            }
+            const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) a[e] *= inv;
+            st<u32x4>(p.O + (long)row * p.so + (long)h * p.ho + 8 * c, pack8(a));
+        }
     }
 }
 
@@ -833,12 +884,12 @@ __global__ __launch_bounds__(256, 2) void pa_dkv_kernel(PAArgs p) {
     }
 }
 
-// dK, dV = sums of the parts; one workgroup = 32 rows of a document, eight columns a thread
+// dK, dV = sums of the parts; eight columns a thread
 __global__ __launch_bounds__(256) void pa_dkv_join_kernel(PAArgs p) {
     const int tile = (int)blockIdx.x % p.nt, d = (int)blockIdx.x / p.nt, w = p.Hkv * DH;
     const Span s = span(p.cu_k, p.len_k, d, p.Tk);
-    for (int r0 = tile * 32; r0 < s.n; r0 += p.nt * 32) {
-        const int rows = min(32, s.n - r0);
+    for (int r0 = tile * JOIN_ROWS; r0 < s.n; r0 += p.nt * JOIN_ROWS) {
+        const int rows = min(JOIN_ROWS, s.n - r0);
         const long base = (long)(s.at + r0) * w;
         for (int i = threadIdx.x; i < rows * (w / 8); i += 256) {
             const long at = base + (long)i * 8;
@@ -865,6 +916,18 @@ __global__ __launch_bounds__(256) void pa_dkv_join_kernel(PAArgs p) {
 
 // ------------------------------------------------------------------------------------------------ host side
 
+// Parts of a query row's keys (inference): as many as bring the workgroups to one per CU, each with four key tiles or more; at most eight, sixteen
+// where that leaves a part 1024 keys.  Whole / in parts, with the join: 890 queries of 16 heads over up to 4097 keys 62 / 44 us (42 + 7 in twice as
+// many parts), 16 queries over 4097 keys 59 / 22 (28 in sixteen), 1 query over 30000 402 / 60 (40 in sixteen), 256 over 1000 20 / 18.
+int fwd_splits_for(int Tq, int H, int max_k, int Tk) {
+    if (max_k <= 0 || max_k > Tk) max_k = Tk;
+    const long wgs = (long)((Tq + 127) / 128) * H;
+    if (wgs < 1) return 1;
+    long s = 256 / wgs;
+    if (s > max_k / 256) s = max_k / 256;
+    const long most = max_k >= 16 * 1024 ? 16 : 8;
+    return (int)(s < 1 ? 1 : s > most ? most : s);
+}
 // Parts of a key tile's sweep: as many as bring the workgroups to twice the chip's 512 slots, at most eight, each with four query tiles or more
 int splits_for(int Tk, int H, int Hkv, int max_q, int Tq) {
     if (max_q <= 0 || max_q > Tq) max_q = Tq;
@@ -937,9 +1000,9 @@ PAArgs common(const void* Q, int64_t sq, int64_t hq, const void* K, int64_t sk, 
 
 int packed_attn_fwd_impl(const void* Q, int64_t sq, int64_t hq, const void* K, int64_t sk, int64_t hk, const void* V, int64_t sv, int64_t hv,
                          const int32_t* cu_q, const int32_t* cu_k, const int32_t* len_q, const int32_t* len_k, const int32_t* prefix, int nd, int Tq,
-                         int Tk, int H, int Hkv, int max_q, int causal, float scale, float softcap, const float* slopes, const float* table,
-                         const int32_t* buckets, int nbuckets, int reach, void* O, int64_t so, int64_t ho, void* Olo, float* lse2, int fill_gaps,
-                         void* stream) {
+                         int Tk, int H, int Hkv, int max_q, int max_k, int causal, float scale, float softcap, const float* slopes, const float* table,
+                         const int32_t* buckets, int nbuckets, int reach, void* O, int64_t so, int64_t ho, void* Olo, float* lse2, float* ws,
+                         int fill_gaps, void* stream) {
     PAArgs a = common(Q, sq, hq, K, sk, hk, V, sv, hv, cu_q, cu_k, len_q, len_k, prefix, nd, Tq, Tk, H, Hkv, causal, scale, softcap, slopes, table,
                       buckets, nbuckets, reach);
     a.O = (bf16_t*)O; a.so = so; a.ho = ho; a.Olo = (bf16_t*)Olo; a.lse2 = lse2; a.fill = fill_gaps;
@@ -948,13 +1011,21 @@ int packed_attn_fwd_impl(const void* Q, int64_t sq, int64_t hq, const void* K, i
     if (rc) return rc;
     if (!O || (!Olo) != (!lse2)) return E2K_ERR_ARG;
     if (!aligned16(Olo)) return E2K_ERR_ALIGN;
+    a.splits = Olo ? 1 : fwd_splits_for(Tq, H, max_k, Tk);
+    a.part = ws;
+    if (a.splits > 1 && !ws) return E2K_ERR_ARG;
     long grid;
-    const int rg = plan_grid(a, max_q, Tq, H, grid);
+    const int rg = plan_grid(a, max_q, Tq, H * a.splits, grid);
     if (rg) return rg;
     if (grid == 0) return E2K_OK;
     hipStream_t st = (hipStream_t)stream;
     PA_PICK(run_fwd, a, Olo != nullptr, grid, st);
     E2K_CHECK_LAUNCH();
+    if (a.splits > 1 && a.nwork > 0) {
+        a.nt *= 128 / JOIN_ROWS;
+        hipLaunchKernelGGL(pa_fwd_join_kernel, dim3((unsigned)(a.nd * a.nt)), dim3(256), 0, st, a);
+        E2K_CHECK_LAUNCH();
+    }
     return E2K_OK;
 }
 
@@ -976,6 +1047,7 @@ int packed_attn_bwd_impl(const void* dO, int64_t sg, int64_t hg, const void* Q, 
         if (!dO || !O || !Olo || !lse2 || !delta || !dQ || (dtable && (!table || !ws))) return E2K_ERR_ARG;
         if (!strides_ok(sg, hg) || !aligned16(dO) || !aligned16(Olo) || !aligned16(dQ) || !aligned16(dK) || !aligned16(dV)) return E2K_ERR_ALIGN;
         if (Tk > 0 && (!dK || !dV)) return E2K_ERR_ARG;
+        a.splits = 1;
         const int rg = plan_grid(a, max_q, Tq, H, grid);
         if (rg) return rg;
         if (grid > 0) {
@@ -1011,7 +1083,7 @@ int packed_attn_bwd_impl(const void* dO, int64_t sg, int64_t hg, const void* Q, 
             E2K_CHECK_LAUNCH();
         }
         if (a.splits > 1 && a.nwork > 0) {
-            a.nt *= 4;                         // 32-row tiles
+            a.nt *= 128 / JOIN_ROWS;
             hipLaunchKernelGGL(pa_dkv_join_kernel, dim3((unsigned)(a.nd * a.nt)), dim3(256), 0, st, a);
             E2K_CHECK_LAUNCH();
         }
@@ -1023,13 +1095,18 @@ int packed_attn_bwd_impl(const void* dO, int64_t sg, int64_t hg, const void* Q, 
 
 extern "C" {
 
+int64_t e2k_query_packed_attn_fwd_ws_floats(int Tq, int Tk, int H, int max_k) {
+    if (Tq < 1 || Tk < 0 || H < 1) return 0;
+    const int s = fwd_splits_for(Tq, H, max_k, Tk);
+    return s > 1 ? (int64_t)s * Tq * H * (DH + 2) : 0;
+}
 int e2k_packed_attn_fwd(const void* Q, int64_t sq, int64_t hq, const void* K, int64_t sk, int64_t hk, const void* V, int64_t sv, int64_t hv,
                         const int32_t* cu_q, const int32_t* cu_k, const int32_t* len_q, const int32_t* len_k, const int32_t* prefix, int nd, int Tq,
-                        int Tk, int H, int Hkv, int max_q, int causal, float scale, float softcap, const float* slopes, const float* table,
-                        const int32_t* buckets, int nbuckets, int reach, void* O, int64_t so, int64_t ho, void* Olo, float* lse2, int fill_gaps,
-                        void* stream) {
+                        int Tk, int H, int Hkv, int max_q, int max_k, int causal, float scale, float softcap, const float* slopes,
+                        const float* table, const int32_t* buckets, int nbuckets, int reach, void* O, int64_t so, int64_t ho, void* Olo, float* lse2,
+                        float* ws, int fill_gaps, void* stream) {
     return e2k::dispatch("packed_attn_fwd", packed_attn_fwd_impl, Q, sq, hq, K, sk, hk, V, sv, hv, cu_q, cu_k, len_q, len_k, prefix, nd, Tq, Tk, H, Hkv,
-                         max_q, causal, scale, softcap, slopes, table, buckets, nbuckets, reach, O, so, ho, Olo, lse2, fill_gaps, stream);
+                         max_q, max_k, causal, scale, softcap, slopes, table, buckets, nbuckets, reach, O, so, ho, Olo, lse2, ws, fill_gaps, stream);
 }
 int64_t e2k_query_packed_attn_bwd_ws_floats(int nd, int Tq, int Tk, int H, int Hkv, int max_q, int reach, int dtable) {
     if (nd < 0 || Tq < 0 || Tk < 0 || H < 1 || Hkv < 1 || H % Hkv != 0 || reach < 0 || reach > REACH_MAX) return 0;

@@ -1151,14 +1151,18 @@ def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, len_q=None, len_k=None, prefix=
     elif out.shape != q.shape or out.dtype != bf16 or out.device != dev or out.stride(2) != 1 or out.stride(0) % 8 or out.stride(1) % 8 or out.data_ptr() % 16 \
             or out.stride(0) >= 1 << 23 or not (out.stride(1) >= 64 and out.stride(0) >= H * 64 or (out.stride(0) >= 64 and out.stride(1) >= Tq * out.stride(0))):
         raise E2KError('packed attention: out must be a (Tq, H, 64) bf16 tensor like q with 16-byte rows that do not overlap')
-    lo = lse2 = None
+    lo = lse2 = ws = None
     if train:
         lo = torch.empty((Tq, H, 64), dtype=bf16, device=dev)
         lse2 = torch.empty((H, Tq), dtype=f32, device=dev)
+    else:
+        n = _lib.get().e2k_query_packed_attn_fwd_ws_floats(Tq, Tk, H, int(max_k))
+        ws = torch.empty(n, dtype=f32, device=dev) if n else None
     with _on_device(q):
         _lib.get().e2k_packed_attn_fwd(_p(q), q.stride(0), q.stride(1), _p(k), k.stride(0), k.stride(1), _p(v), v.stride(0), v.stride(1), _p(cu_q), _p(cu_k),
-                                       _p(len_q), _p(len_k), _p(prefix), nd, Tq, Tk, H, Hkv, int(max_q), int(bool(causal)), scale, softcap, _p(slopes),
-                                       _p(table), _p(buckets), nb, reach, _p(out), out.stride(0), out.stride(1), _p(lo), _p(lse2), int(fill), _stream(q))
+                                       _p(len_q), _p(len_k), _p(prefix), nd, Tq, Tk, H, Hkv, int(max_q), int(max_k), int(bool(causal)), scale,
+                                       softcap, _p(slopes), _p(table), _p(buckets), nb, reach, _p(out), out.stride(0), out.stride(1), _p(lo), _p(lse2),
+                                       _p(ws), int(fill), _stream(q))
     if not train:
         return out
     st = PackedAttnState()

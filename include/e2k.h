@@ -357,12 +357,14 @@ int e2k_freq_attn_bwd(const void* dout, const void* qkv, int64_t ld, const void*
  * slopes / table or neither), softmax over the visible keys, O = P V; a row that sees nothing is 0.  A bias of -1e30 or less hides its keys.
  * O (Tq, H, 64) strided; rows that no document covers are zeroed with fill_gaps = 1, left alone with 0.  For the backward: Olo
  * (Tq, H, 64) contiguous (what rounding to bf16 cut off O) and lse2 (H, Tq) fp32 (log2 domain), both or neither.
- * max_q (max_k): the longest document, a sizing hint -- longer ones are computed all the same; 0 = unknown. */
+ * max_q (max_k): the longest document, a sizing hint -- longer ones are computed all the same; 0 = unknown.
+ * ws: e2k_query_packed_attn_fwd_ws_floats floats, 16-byte aligned, without Olo (0, or with Olo: NULL will do). */
+int64_t e2k_query_packed_attn_fwd_ws_floats(int Tq, int Tk, int H, int max_k);
 int e2k_packed_attn_fwd(const void* Q, int64_t sq, int64_t hq, const void* K, int64_t sk, int64_t hk, const void* V, int64_t sv, int64_t hv,
                         const int32_t* cu_q, const int32_t* cu_k, const int32_t* len_q, const int32_t* len_k, const int32_t* prefix, int nd,
-                        int Tq, int Tk, int H, int Hkv, int max_q, int causal, float scale, float softcap, const float* slopes,
+                        int Tq, int Tk, int H, int Hkv, int max_q, int max_k, int causal, float scale, float softcap, const float* slopes,
                         const float* table, const int32_t* buckets, int nbuckets, int reach, void* O, int64_t so, int64_t ho, void* Olo,
-                        float* lse2, int fill_gaps, void* stream);
+                        float* lse2, float* ws, int fill_gaps, void* stream);
 /* dQ (Tq, H, 64), dK, dV (Tk, Hkv, 64) contiguous (uncovered rows as above); delta (H, Tq) scratch.  dtable (may be NULL): gradient of the table,
  * (nbuckets, H) fp32, added to with accumulate = 1.
  * ws: e2k_query_packed_attn_bwd_ws_floats floats, 16-byte aligned (0: NULL will do).  Deterministic. */

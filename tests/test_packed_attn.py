@@ -504,3 +504,21 @@ def test_packed_attention_split_sweep(dev, mask, bias):
     assert (got['dk'][65:70] == 0).all() and (got['dv'][170:] == 0).all()
     again = run(c, dev, max_q=600)
     assert all(torch.equal(got[n], again[n]) for n in got)
+
+
+@pytest.mark.parametrize('bias', BIASES)
+@pytest.mark.parametrize('mask', ['full', 'causal'])
+def test_packed_attention_split_keys(dev, mask, bias):
+    """inference with few queries over many keys: a row's keys in parts, some of them empty; queries that see nothing; gaps between the documents"""
+    from e2_tts_pytorch_amd import _lib, ops
+    c = Case([70, 8, 10], kl=[700, 3, 40], H=2, nq=[65, 8, 10], nk=[650, 3, 40], mask=mask, bias=bias, cap=20., tail=3)
+    assert _lib.get().e2k_query_packed_attn_fwd_ws_floats(c.q.shape[0], c.k.shape[0], c.H, 700) > 0
+    want, bound = c.exact()
+    a, kw = c.args(dev)
+    out = ops.packed_attn_fwd(*a, max_k=700, **kw)
+    held(out, want['out'], bound['out'], 'out')
+    assert (out[65:70] == 0).all() and (out[88:] == 0).all() and (mask == 'full' or (out[70:75] == 0).all())
+    assert torch.equal(out, ops.packed_attn_fwd(*a, max_k=700, **kw))
+    buf = torch.full((c.q.shape[0], 2, 64), 7., dtype=bf16, device=dev)
+    ops.packed_attn_fwd(*a, max_k=700, out=buf, **kw)
+    assert (buf[65:70] == 7).all() and (buf[88:] == 7).all() and torch.equal(buf[:65], out[:65])
