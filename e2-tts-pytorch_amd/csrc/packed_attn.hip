@@ -777,10 +777,12 @@ __global__ __launch_bounds__(256, 2) void pa_dkv_kernel(PAArgs p) {
             if (it + 2 < total) issue(it + 2);
             if (BIAS == 1 && p.G > 1 && j0 == 0 && it > 0) sc.init(p, p.slopes[wk.h * p.G + hd]);
             if (BIAS == 2) {
-                float* L = lut + (hd & 1) * distn(REACH_MAX);
-                sc.lut = L;
-                sc.far_lo = L[PADL];
-                sc.far_hi = L[PADL + 2 * p.R];
+                if (j0 == 0 || it == 0) {                     // (its LDS reads wait for every copy in flight: once a head, not once a tile)
+                    float* L = lut + (hd & 1) * distn(REACH_MAX);
+                    sc.lut = L;
+                    sc.far_lo = L[PADL];
+                    sc.far_hi = L[PADL + 2 * p.R];
+                }
                 // the next head's table while this head's last tile is computed (the other buffer: its last reader passed the barrier above)
                 if (j0 == per - 1 && hd + 1 < p.G) {
                     load_lut(p, wk.h * p.G + hd + 1, lut + ((hd + 1) & 1) * distn(REACH_MAX));
@@ -953,16 +955,29 @@ int check(const PAArgs& a) {
     if (!aligned16(a.Q) || !aligned16(a.K) || !aligned16(a.V) || !aligned16(a.O)) return E2K_ERR_ALIGN;
     return E2K_OK;
 }
-// grid of `rows`-row problems: tiles per (document, head) and workgroups
-int plan_grid(PAArgs& a, int longest, int total, int heads, long& grid) {
+// 128-row tiles per (document, head) of a grid: those of the longest document, fewer where documents x heads would make the grid absurd (every
+// document gets as many workgroups as the longest is thought to need; a workgroup takes further tiles of its document in turn)
+int tiles_for(int longest, int total, int nd, int heads) {
     if (longest <= 0 || longest > total) longest = total;
-    a.nt = (longest + 127) / 128;
-    if (a.nt < 1) a.nt = 1;
+    const long most = 262144 / ((long)(nd > 0 ? nd : 1) * heads);
+    long nt = ((long)longest + 127) / 128;
+    if (nt > most) nt = most;
+    return (int)(nt < 1 ? 1 : nt);
+}
+int plan_grid(PAArgs& a, int longest, int total, int heads, long& grid) {
+    a.nt = tiles_for(longest, total, a.nd, heads);
     const long work = (long)a.nd * a.nt * heads;
-    grid = work + (a.fill ? (long)(a.nd + 1) * GAP_PARTS : 0);
+    grid = work + (a.fill ? ((long)a.nd + 1) * GAP_PARTS : 0);
     if (grid > 0x7fffffffL / 256) return E2K_ERR_SHAPE;
     a.nwork = (int)work;
     return E2K_OK;
+}
+// the same rows in JOIN_ROWS-row tiles
+void plan_join(PAArgs& a) {
+    const long most = 65536 / a.nd;
+    long nt = (long)a.nt * (128 / JOIN_ROWS);
+    if (nt > most) nt = most;
+    a.nt = (int)(nt < 1 ? 1 : nt);
 }
 
 template <int BIAS, bool CAP> void run_fwd(const PAArgs& a, bool train, long grid, hipStream_t st) {
@@ -1022,7 +1037,7 @@ int packed_attn_fwd_impl(const void* Q, int64_t sq, int64_t hq, const void* K, i
     PA_PICK(run_fwd, a, Olo != nullptr, grid, st);
     E2K_CHECK_LAUNCH();
     if (a.splits > 1 && a.nwork > 0) {
-        a.nt *= 128 / JOIN_ROWS;
+        plan_join(a);
         hipLaunchKernelGGL(pa_fwd_join_kernel, dim3((unsigned)(a.nd * a.nt)), dim3(256), 0, st, a);
         E2K_CHECK_LAUNCH();
     }
@@ -1059,7 +1074,7 @@ int packed_attn_bwd_impl(const void* dO, int64_t sg, int64_t hg, const void* Q, 
     }
     float* rest = ws;                          // workspace behind the table's part
     if (dtable) {
-        if (!table || !ws || nbuckets < 1 || reach < 0 || reach > REACH_MAX) return E2K_ERR_ARG;
+        if (!table || !buckets || !ws || nbuckets < 1 || reach < 0 || reach > REACH_MAX) return E2K_ERR_ARG;
         const int N = 2 * reach + 1;
         const long nq_work = a.nwork;
         float* by_dist = ws + (Tq > 0 ? nq_work * N : 0);
@@ -1083,7 +1098,7 @@ int packed_attn_bwd_impl(const void* dO, int64_t sg, int64_t hg, const void* Q, 
             E2K_CHECK_LAUNCH();
         }
         if (a.splits > 1 && a.nwork > 0) {
-            a.nt *= 128 / JOIN_ROWS;
+            plan_join(a);
             hipLaunchKernelGGL(pa_dkv_join_kernel, dim3((unsigned)(a.nd * a.nt)), dim3(256), 0, st, a);
             E2K_CHECK_LAUNCH();
         }
@@ -1113,9 +1128,8 @@ int64_t e2k_query_packed_attn_bwd_ws_floats(int nd, int Tq, int Tk, int H, int H
     const int s = splits_for(Tk, H, Hkv, max_q, Tq);
     const int64_t join = s > 1 ? (int64_t)s * 2 * Tk * Hkv * DH : 0;
     if (!dtable) return join;
-    if (max_q <= 0 || max_q > Tq) max_q = Tq;
-    const int64_t nt = max_q > 0 ? (max_q + 127) / 128 : 1;
-    const int64_t sums = ((Tq > 0 ? nd * nt * H : 0) + H) * (2 * (int64_t)reach + 1);
+    const int64_t wgs = Tq > 0 ? (int64_t)nd * tiles_for(max_q, Tq, nd, H) * H : 0;
+    const int64_t sums = (wgs + H) * (2 * (int64_t)reach + 1);
     return (sums + 3) / 4 * 4 + join;
 }
 int e2k_packed_attn_bwd(const void* dO, int64_t sg, int64_t hg, const void* Q, int64_t sq, int64_t hq, const void* K, int64_t sk, int64_t hk,

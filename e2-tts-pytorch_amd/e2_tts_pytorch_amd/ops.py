@@ -78,6 +78,23 @@ class pinned_stream:
         return False
 
 
+class _on_device:
+    """kernels launch on the device of their tensors, whichever is current"""
+    __slots__ = ('guard',)
+
+    def __init__(self, t):
+        self.guard = torch.cuda.device(t.device) if t.is_cuda and t.device.index != torch.cuda.current_device() else None
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+        return False
+
+
 def lib():
     return _lib.get()
 
@@ -633,13 +650,18 @@ def rmsnorm_bwd(dy, x, rn, gamma, gamma_off, rows_per_batch, dgamma):
     return dx
 
 
-def _ln_cols(t, M, D, rows_per_batch, what):
-    """checks a (D,) or (batch elements, D) fp32 column vector of a layer norm -> 2-D view"""
+def _ln_cols(t, x, rows_per_batch, what, written=False):
+    """checks a (D,) or (batch elements, D) fp32 column vector of a layer norm over x -> 2-D view (a copy where rows are broadcast)"""
+    M, D = x.shape
     if t.dim() == 1:
         t = t[None]
     need = -(-M // rows_per_batch)
-    if t.dtype != f32 or t.dim() != 2 or t.shape[1] != D or t.shape[0] < need or (D > 1 and t.stride(1) != 1):
-        raise E2KError(f'layer norm: {what} must be fp32 ({need} or more, {D}) with contiguous rows, got {t.dtype} {tuple(t.shape)}')
+    if t.dtype != f32 or t.dim() != 2 or t.shape[1] != D or t.shape[0] < need or (D > 1 and t.stride(1) != 1) or t.device != x.device:
+        raise E2KError(f'layer norm: {what} must be fp32 ({need} or more, {D}) with contiguous rows on the device of x, got {t.dtype} {tuple(t.shape)}')
+    if t.shape[0] > 1 and t.stride(0) < D:
+        if written:
+            raise E2KError(f'layer norm: rows of {what} overlap')
+        t = t.contiguous()
     return t
 
 
@@ -660,16 +682,16 @@ def layernorm_fwd(x, gamma, beta, gamma_off=0., rows_per_batch=0, eps=1e-5):
     rpb = int(rows_per_batch) or max(M, 1)
     if rpb < 0 or not eps >= 0:
         raise E2KError('layer norm: rows_per_batch and eps must not be negative')
-    gamma = None if gamma is None else _ln_cols(gamma, M, D, rpb, 'gamma')
-    beta = None if beta is None else _ln_cols(beta, M, D, rpb, 'beta')
-    if gamma is not None and beta is not None and gamma.shape[0] > 1 and gamma.stride(0) != beta.stride(0):
-        beta = beta.contiguous()
-        gamma = gamma.contiguous()
+    gamma = None if gamma is None else _ln_cols(gamma, x, rpb, 'gamma')
+    beta = None if beta is None else _ln_cols(beta, x, rpb, 'beta')
+    if gamma is not None and beta is not None and gamma.stride(0) != beta.stride(0):
+        gamma, beta = gamma.contiguous(), beta.contiguous()
     ldg = next((t.stride(0) for t in (gamma, beta) if t is not None), D)
     y = torch.empty((M, D), dtype=x.dtype, device=x.device)
     mean, rstd = (torch.empty(M, dtype=f32, device=x.device) for _ in range(2))
-    _lib.get().e2k_layernorm_fwd(_p(x), ldx, int(x.dtype == f32), _p(gamma), _p(beta), ldg, float(gamma_off), rpb, float(eps), _p(y), _p(mean), _p(rstd),
-                                 M, D, _stream(x))
+    with _on_device(x):
+        _lib.get().e2k_layernorm_fwd(_p(x), ldx, int(x.dtype == f32), _p(gamma), _p(beta), ldg, float(gamma_off), rpb, float(eps), _p(y), _p(mean),
+                                     _p(rstd), M, D, _stream(x))
     return y, mean, rstd
 
 
@@ -681,13 +703,13 @@ def layernorm_bwd(dy, x, mean, rstd, gamma, gamma_off=0., rows_per_batch=0, dgam
     M, D = x.shape
     rpb = int(rows_per_batch) or max(M, 1)
     nb = -(-M // rpb)
-    if dy.shape != x.shape or dy.dtype != x.dtype:
+    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
         raise E2KError(f'layer norm: dy must match x, got {dy.dtype} {tuple(dy.shape)} for {x.dtype} {tuple(x.shape)}')
     dy = dy.contiguous()
     for t in (mean, rstd):
-        if t.dtype != f32 or t.shape != (M,) or not t.is_contiguous():
+        if t.dtype != f32 or t.shape != (M,) or not t.is_contiguous() or t.device != x.device:
             raise E2KError('layer norm: mean and rstd are the forward\'s')
-    gamma = None if gamma is None else _ln_cols(gamma, M, D, rpb, 'gamma')
+    gamma = None if gamma is None else _ln_cols(gamma, x, rpb, 'gamma')
     dx = torch.empty((M, D), dtype=x.dtype, device=x.device)
     ws, ldd, acc = None, D, 0
     if need_weights:
@@ -697,17 +719,16 @@ def layernorm_bwd(dy, x, mean, rstd, gamma, gamma_off=0., rows_per_batch=0, dgam
             dgamma, dbeta = (torch.zeros if M == 0 else torch.empty)((2, nb, D), dtype=f32, device=x.device).unbind(0)
         else:
             acc = 1
-            _ln_cols(dgamma, M, D, rpb, 'dgamma'), _ln_cols(dbeta, M, D, rpb, 'dbeta')
+            _ln_cols(dgamma, x, rpb, 'dgamma', True), _ln_cols(dbeta, x, rpb, 'dbeta', True)
             if dgamma.shape != dbeta.shape or dgamma.stride() != dbeta.stride():
                 raise E2KError('layer norm: dgamma and dbeta must have the same shape and strides')
-            if dgamma.dim() == 2 and dgamma.shape[0] > 1 and dgamma.stride(0) < D:
-                raise E2KError('layer norm: rows of dgamma overlap')
         ldd = dgamma.stride(0) if dgamma.dim() == 2 else D
         ws = torch.empty(_lib.get().e2k_query_layernorm_bwd_ws_floats(M, D, rpb), dtype=f32, device=x.device)
     elif dgamma is not None or dbeta is not None:
         raise E2KError('layer norm: dgamma / dbeta given with need_weights=False')
-    _lib.get().e2k_layernorm_bwd(_p(dy), _p(x), ldx, int(x.dtype == f32), _p(mean), _p(rstd), _p(gamma), gamma.stride(0) if gamma is not None else D,
-                                 float(gamma_off), rpb, _p(dx), _p(dgamma), _p(dbeta), ldd, acc, _p(ws), M, D, _stream(x))
+    with _on_device(x):
+        _lib.get().e2k_layernorm_bwd(_p(dy), _p(x), ldx, int(x.dtype == f32), _p(mean), _p(rstd), _p(gamma), gamma.stride(0) if gamma is not None else D,
+                                     float(gamma_off), rpb, _p(dx), _p(dgamma), _p(dbeta), ldd, acc, _p(ws), M, D, _stream(x))
     return dx, dgamma, dbeta
 
 
@@ -1031,23 +1052,6 @@ def qkv_post_bwd(st, dQ, dK, dV, dgate_pre, qkvg, cosb, sinb, vfirst=None, dvfir
 
 
 # ------------------------------------------------------------------------------------------------ attention over packed documents
-
-class _on_device:
-    """kernels launch on the device of their tensors, whichever is current"""
-    __slots__ = ('guard',)
-
-    def __init__(self, t):
-        self.guard = torch.cuda.device(t.device) if t.is_cuda and t.device.index != torch.cuda.current_device() else None
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-        return False
-
 
 def _heads64(t, what):
     """(tokens, heads, 64) bf16 that the kernels can read in place (16-byte rows, strides they can address), a contiguous copy otherwise"""

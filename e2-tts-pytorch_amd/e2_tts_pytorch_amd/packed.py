@@ -49,6 +49,8 @@ def packed_attention(q, k, v, cu_q, cu_k=None, *, len_q=None, len_k=None, prefix
         raise ops.E2KError('packed_attention: slopes get no gradient; pass slopes.detach(), or learn a RelativePositionBias')
     table, buckets = (None, None) if bias is None else (bias.weight, bias.buckets)
     kw = dict(len_q=len_q, len_k=len_k, prefix=prefix, max_q=max_q, max_k=max_k, causal=causal, scale=scale, softcap=softcap, slopes=slopes, buckets=buckets)
+    if not torch.is_grad_enabled():              # (nothing is kept for a backward)
+        return ops.packed_attn_fwd(q, k, v, cu_q, cu_k, table=table, **kw)
     return _PackedAttnFn.apply(q, k, v, table, cu_q, cu_k, kw)
 
 

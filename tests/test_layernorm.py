@@ -168,3 +168,20 @@ def test_layer_norm_refusals(emu):
         with pytest.raises(ops.E2KError):
             f()
             print('not refused:', i)
+
+
+def test_layer_norm_broadcast_columns(dev):
+    """scale and shift expanded over the batch elements, or with strides of their own, are read as they stand"""
+    from e2_tts_pytorch_amd import ops
+    x, dy, gamma, beta = (t.to(dev) for t in inputs(8, 96, 1, f32))
+    want = ops.layernorm_fwd(x, gamma, beta, 1., 0)[0]
+    wide = torch.zeros(4, 200, device=dev)
+    wide[:, :96] = beta
+    assert torch.equal(ops.layernorm_fwd(x, gamma.expand(4, 96), wide[:, :96], 1., 2)[0], want)
+    y, m, r = ops.layernorm_fwd(x, gamma.expand(4, 96), beta.expand(4, 96), 1., 2)
+    assert torch.equal(y, want)
+    dx, dg, db = ops.layernorm_bwd(dy, x, m, r, gamma.expand(4, 96), 1., 2)
+    one = ops.layernorm_bwd(dy, x, m, r, gamma, 1., 0)
+    assert torch.equal(dx, one[0]) and (dg.sum(0) - one[1][0]).abs().max() < 1e-4
+    with pytest.raises(ops.E2KError):
+        ops.layernorm_bwd(dy, x, m, r, gamma, 1., 2, torch.zeros(1, 96, device=dev).expand(4, 96), torch.zeros(1, 96, device=dev).expand(4, 96))

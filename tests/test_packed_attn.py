@@ -522,3 +522,22 @@ def test_packed_attention_split_keys(dev, mask, bias):
     buf = torch.full((c.q.shape[0], 2, 64), 7., dtype=bf16, device=dev)
     ops.packed_attn_fwd(*a, max_k=700, out=buf, **kw)
     assert (buf[65:70] == 7).all() and (buf[88:] == 7).all() and torch.equal(buf[:65], out[:65])
+
+
+def test_packed_attention_many_documents(dev):
+    """more documents x heads than the grid has tiles for: a workgroup takes several tiles of its document (the sums by distance too)"""
+    from e2_tts_pytorch_amd import _lib, ops
+    n = 70000 if gpu_shapes(dev) else 9000
+    lens = [0] * n
+    lens[5], lens[n - 3] = 300, 40
+    H = 2 if gpu_shapes(dev) else 16
+    c = Case([300, 40], H=H, bias='table')
+    want, bound = c.exact()
+    a, kw = c.args(dev)
+    cu = torch.zeros(n + 1, dtype=torch.int32)
+    cu[6:], cu[n - 2:] = 300, 340
+    cu = cu.to(dev)
+    out, st = ops.packed_attn_fwd(a[0], a[1], a[2], cu, train=True, **kw)
+    dq, dk, dv, dtable = ops.packed_attn_bwd(st, c.dout.to(dev))
+    for name, t in (('out', out), ('dq', dq), ('dk', dk), ('dv', dv), ('dtable', dtable)):
+        held(t, want[name], bound[name], name)
