@@ -6,7 +6,7 @@
 // What bounds it: HBM (x and y once; x, dy and dx once).  A row stays in registers between its two reductions (mean first, then the
 // centred squares: no cancellation however far the mean lies from 0); the next row of the wave is loaded while the current one is
 // reduced.  64 lanes own a row up to 1536 columns, 256 lanes beyond (up to 8192).  Rows whose addresses or width are not multiples of
-// 16 bytes take element-wise accesses (still whole lines per wave instruction).
+// 16 bytes take the same accesses unaligned, the last few columns one by one (element-wise rows reached 3.8 TB/s at 16399 x 1003 fp32).
 // The sums over rows of the backward stay in registers over all rows of a wave, are joined in LDS in a fixed order, and leave as one
 // partial row per workgroup; a second kernel adds the partials in a fixed order: no atomics, the same bits every time.
 #include "e2k_device.h"
@@ -33,68 +33,89 @@ struct LNArgs {
     int gpb;                            // backward: workgroups per batch element
 };
 
-// E elements of a row per lane: chunk c holds columns (c LPR + t) VEC .. + VEC - 1 of the row
-template <class T, int VEC, int NCH, int LPR> struct Row {
-    static constexpr int E = VEC * NCH;
-    static constexpr int RAW = (E * (int)sizeof(T) + 3) / 4;
-    unsigned w[VEC == 1 ? E : RAW];     // raw bits (element-wise rows: one element a register)
+// vectors at any element's alignment (gfx950 loads and stores 16 bytes at any address; the type keeps the compiler from assuming more)
+typedef u32x4 u32x4_u __attribute__((aligned(2)));
+typedef f32x4 f32x4_u __attribute__((aligned(4)));
+
+// E elements of a row per lane: chunk c holds columns (c LPR + t) VEC .. + VEC - 1 of the row; columns past the end read 0.
+// AL: rows start on 16 bytes and are whole vectors
+template <class T, int NCH, int LPR, bool AL> struct Row {
+    static constexpr int VEC = 16 / (int)sizeof(T), E = VEC * NCH;
+    u32x4 w[NCH];
 
     __device__ __forceinline__ void load(const T* row, int t, int D) {
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
             const int col = (c * LPR + t) * VEC;
-            if (VEC == 1) {
-                w[c] = 0u;
-                if (col < D) w[c] = sizeof(T) == 2 ? (unsigned)*(const bf16_t*)(row + col) << 16 : *(const unsigned*)(row + col);
+            u32x4 v = {0u, 0u, 0u, 0u};
+            if (AL) {
+                if (col < D) v = ld<u32x4>(row + col);
+            } else if (col + VEC <= D) {
+                v = *(const u32x4_u*)(row + col);
             } else {
-                const u32x4 v = col < D ? ld<u32x4>(row + col) : u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[4 * c + i] = v[i];
+                for (int i = 0; i < VEC; ++i)
+                    if (col + i < D) {
+                        if (sizeof(T) == 2) v[i >> 1] |= (unsigned)*(const bf16_t*)(row + col + i) << (16 * (i & 1));
+                        else v[i] = *(const unsigned*)(row + col + i);
+                    }
             }
+            w[c] = v;
         }
     }
     __device__ __forceinline__ float get(int e) const {
-        if (VEC == 1 || sizeof(T) == 4) return __uint_as_float(w[e]);
-        return (e & 1) ? bfhi(w[e >> 1]) : bflo(w[e >> 1]);
+        if (sizeof(T) == 4) return __uint_as_float(w[e >> 2][e & 3]);
+        return (e & 1) ? bfhi(w[e >> 3][(e & 7) >> 1]) : bflo(w[e >> 3][(e & 7) >> 1]);
     }
 };
-template <class T, int VEC, int NCH, int LPR>
-__device__ __forceinline__ void store_elems(T* row, int t, int D, const float (&v)[VEC * NCH]) {
+template <class T, int NCH, int LPR, bool AL>
+__device__ __forceinline__ void store_elems(T* row, int t, int D, const float (&v)[16 / (int)sizeof(T) * NCH]) {
+    constexpr int VEC = 16 / (int)sizeof(T);
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
         const int col = (c * LPR + t) * VEC;
         if (col >= D) continue;
-        if (VEC == 1) {
-            if (sizeof(T) == 2) *(bf16_t*)(row + col) = f2bf(v[c]);
-            else *(float*)(row + col) = v[c];
-        } else if (sizeof(T) == 2) {
-            st<u32x4>(row + col, pack8(&v[VEC * c]));
+        u32x4 q;
+        if (sizeof(T) == 2) q = pack8(&v[VEC * c]);
+        else q = __builtin_bit_cast(u32x4, f32x4{v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]});
+        if (AL) {
+            st<u32x4>(row + col, q);
+        } else if (col + VEC <= D) {
+            *(u32x4_u*)(row + col) = q;
         } else {
-            st<f32x4>(row + col, f32x4{v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]});
+#pragma unroll
+            for (int i = 0; i < VEC; ++i)
+                if (col + i < D) {
+                    if (sizeof(T) == 2) *(bf16_t*)(row + col + i) = (bf16_t)(q[i >> 1] >> (16 * (i & 1)));
+                    else *(unsigned*)(row + col + i) = q[i];
+                }
         }
     }
 }
-// per-column fp32 vector (gamma / beta), 16 bytes at a time where the rows are; `none` where there is none
-template <int VEC, int NCH, int LPR>
+// per-column fp32 vector (gamma / beta); `none` where there is none
+template <int VEC, int NCH, int LPR, bool AL>
 __device__ __forceinline__ void load_cols(const float* p, float off, float none, int t, int D, float (&v)[VEC * NCH]) {
 #pragma unroll
     for (int e = 0; e < VEC * NCH; ++e) v[e] = none;
     if (!p) return;
 #pragma unroll
-    for (int c = 0; c < NCH; ++c) {
-        const int col = (c * LPR + t) * VEC;
-        if (col >= D) continue;
-        if (VEC == 1) {
-            v[c] = p[col] + off;
-        } else {
+    for (int c = 0; c < NCH; ++c)
 #pragma unroll
-            for (int i = 0; i < VEC; i += 4) {
-                const f32x4 w = ld<f32x4>(p + col + i);
+        for (int i = 0; i < VEC; i += 4) {
+            const int col = (c * LPR + t) * VEC + i;
+            f32x4 w = {0.f, 0.f, 0.f, 0.f};
+            if (AL) {
+                if (col < D) w = ld<f32x4>(p + col);
+            } else if (col + 4 <= D) {
+                w = *(const f32x4_u*)(p + col);
+            } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[c * VEC + i + j] = w[j] + off;
+                for (int j = 0; j < 4; ++j)
+                    if (col + j < D) w[j] = p[col + j];
             }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[c * VEC + i + j] = w[j] + off;
         }
-    }
 }
 
 // sums over the LPR lanes of a row; with 256 lanes every wave of the workgroup takes part (buf: 2 floats per wave, double-buffered by `ph`)
@@ -112,27 +133,27 @@ template <int LPR> __device__ __forceinline__ void row_sum2(float& a, float& b, 
 }
 
 // A workgroup of four waves; a row slot (wave, or the whole workgroup) takes rows slot, slot + nslots, ... of its contiguous share.
-template <class T, int VEC, int NCH, int LPR>
+template <class T, int NCH, int LPR, bool AL>
 __global__ __launch_bounds__(256) void ln_fwd_kernel(LNArgs p, int share) {
-    constexpr int E = VEC * NCH, RPW = 256 / LPR;
+    constexpr int VEC = 16 / (int)sizeof(T), E = VEC * NCH, RPW = 256 / LPR;
     __shared__ float buf[4 * LN_WAVES];
     const int wave = uniform_i(threadIdx.x >> 6), t = threadIdx.x & (LPR - 1), slot = LPR == 64 ? wave : 0;
     const long r0 = (long)blockIdx.x * share * RPW + slot;
     float w[E], b[E];
     int cur = -1;
-    Row<T, VEC, NCH, LPR> nx;
+    Row<T, NCH, LPR, AL> nx;
     if (r0 < p.M) nx.load((const T*)p.x + r0 * p.ldx, t, p.D);
     const float inv = 1.f / (float)p.D;
     for (int s = 0; s < share; ++s) {
         const long r = r0 + (long)s * RPW;
         if (r >= p.M) break;           // (uniform over the lanes that meet in a reduction: a wave, or the workgroup that is one row slot)
-        const Row<T, VEC, NCH, LPR> x = nx;
+        const Row<T, NCH, LPR, AL> x = nx;
         if (s + 1 < share && r + RPW < p.M) nx.load((const T*)p.x + (r + RPW) * p.ldx, t, p.D);
         const int bi = (int)((unsigned)r / (unsigned)p.rpb);
         if (bi != cur) {
             cur = bi;
-            load_cols<VEC, NCH, LPR>(p.gamma ? p.gamma + bi * p.ldg : nullptr, p.gamma_off, 1.f, t, p.D, w);
-            load_cols<VEC, NCH, LPR>(p.beta ? p.beta + bi * p.ldg : nullptr, 0.f, 0.f, t, p.D, b);
+            load_cols<VEC, NCH, LPR, AL>(p.gamma ? p.gamma + bi * p.ldg : nullptr, p.gamma_off, 1.f, t, p.D, w);
+            load_cols<VEC, NCH, LPR, AL>(p.beta ? p.beta + bi * p.ldg : nullptr, 0.f, 0.f, t, p.D, b);
         }
         float m = 0.f, z = 0.f;
 #pragma unroll
@@ -151,28 +172,28 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(LNArgs p, int share) {
         const float rs = 1.f / sqrtf(fmaf(q, inv, p.eps));
 #pragma unroll
         for (int e = 0; e < E; ++e) v[e] = fmaf(v[e] * rs, w[e], b[e]);
-        store_elems<T, VEC, NCH, LPR>((T*)p.y + r * (long)p.D, t, p.D, v);
+        store_elems<T, NCH, LPR, AL>((T*)p.y + r * (long)p.D, t, p.D, v);
         if (t == 0 && p.mean) { p.mean[r] = m; p.rstd[r] = rs; }
     }
 }
 
 // Workgroup g of batch element b takes every gpb-th block of eight (two) rows of it; its column sums go to ws[b gpb + g].
-template <class T, int VEC, int NCH, int LPR>
+template <class T, int NCH, int LPR, bool AL>
 __global__ __launch_bounds__(64 * LN_WAVES) void ln_bwd_kernel(LNArgs p) {
-    constexpr int E = VEC * NCH, SLOTS = LN_WAVES * 64 / LPR;
+    constexpr int VEC = 16 / (int)sizeof(T), E = VEC * NCH, SLOTS = LN_WAVES * 64 / LPR;
     __shared__ float sm[(SLOTS / 2) * 2 * E * LPR];             // [slot][dgamma | dbeta][element][lane]: at most 64 KB
     __shared__ float buf[4 * LN_WAVES];
     const int wave = uniform_i(threadIdx.x >> 6), t = threadIdx.x & (LPR - 1), slot = LPR == 64 ? wave : wave >> 2;
     const int bi = blockIdx.x / p.gpb, g = blockIdx.x % p.gpb;
     const long first = (long)bi * p.rpb, last = first + p.rpb < p.M ? first + p.rpb : p.M;
     float w[E], sg[E], sb[E];
-    load_cols<VEC, NCH, LPR>(p.gamma ? p.gamma + bi * p.ldg : nullptr, p.gamma_off, 1.f, t, p.D, w);
+    load_cols<VEC, NCH, LPR, AL>(p.gamma ? p.gamma + bi * p.ldg : nullptr, p.gamma_off, 1.f, t, p.D, w);
 #pragma unroll
     for (int e = 0; e < E; ++e) { sg[e] = 0.f; sb[e] = 0.f; }
     const float inv = 1.f / (float)p.D;
     const long step = (long)p.gpb * SLOTS;
     long r = first + (long)g * SLOTS + slot;
-    Row<T, VEC, NCH, LPR> nx, nd;
+    Row<T, NCH, LPR, AL> nx, nd;
     float nm = 0.f, nr = 0.f;
     auto fetch = [&](long row) __attribute__((always_inline)) {
         nx.load((const T*)p.x + row * p.ldx, t, p.D);
@@ -185,7 +206,7 @@ __global__ __launch_bounds__(64 * LN_WAVES) void ln_bwd_kernel(LNArgs p) {
     for (long base = first + (long)g * SLOTS; base < last; base += step, r += step) {
         const bool in = r < last;
         if (LPR == 64 && !in) break;
-        const Row<T, VEC, NCH, LPR> x = nx, d = nd;
+        const Row<T, NCH, LPR, AL> x = nx, d = nd;
         const float m = nm, rs = in ? nr : 0.f;
         if (r + step < last) fetch(r + step);
         float xh[E], gy[E], c1 = 0.f, c2 = 0.f;
@@ -206,7 +227,7 @@ __global__ __launch_bounds__(64 * LN_WAVES) void ln_bwd_kernel(LNArgs p) {
             float v[E];
 #pragma unroll
             for (int e = 0; e < E; ++e) v[e] = rs * (gy[e] - c1 - xh[e] * c2);
-            store_elems<T, VEC, NCH, LPR>((T*)p.y + r * (long)p.D, t, p.D, v);
+            store_elems<T, NCH, LPR, AL>((T*)p.y + r * (long)p.D, t, p.D, v);
         }
     }
     if (!p.ws) return;
@@ -269,35 +290,35 @@ int fwd_share(int M, int rpw) {
     return (int)(s < 1 ? 1 : s > 16 ? 16 : s);
 }
 
-template <class T, int VEC, int NCH, int LPR> int launch_fwd(const LNArgs& a, hipStream_t st) {
+template <class T, int NCH, int LPR, bool AL> int launch_fwd(const LNArgs& a, hipStream_t st) {
     constexpr int RPW = 256 / LPR;
     const int share = fwd_share(a.M, RPW);
     const long per = (long)share * RPW;
-    hipLaunchKernelGGL((ln_fwd_kernel<T, VEC, NCH, LPR>), dim3((unsigned)((a.M + per - 1) / per)), dim3(256), 0, st, a, share);
+    hipLaunchKernelGGL((ln_fwd_kernel<T, NCH, LPR, AL>), dim3((unsigned)((a.M + per - 1) / per)), dim3(256), 0, st, a, share);
     E2K_CHECK_LAUNCH();
     return E2K_OK;
 }
-template <class T, int VEC, int NCH, int LPR> int launch_bwd(const LNArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL((ln_bwd_kernel<T, VEC, NCH, LPR>), dim3(a.nb * a.gpb), dim3(64 * LN_WAVES), 0, st, a);
+template <class T, int NCH, int LPR, bool AL> int launch_bwd(const LNArgs& a, hipStream_t st) {
+    hipLaunchKernelGGL((ln_bwd_kernel<T, NCH, LPR, AL>), dim3(a.nb * a.gpb), dim3(64 * LN_WAVES), 0, st, a);
     E2K_CHECK_LAUNCH();
     return E2K_OK;
 }
 
 // widths per instantiation: columns a row's lanes cover
-#define LN_PICK(FN, T, VEC)                                                                       \
+#define LN_PICK(FN, T, AL)                                                                        \
     do {                                                                                          \
-        constexpr int V_ = VEC;                                                                   \
+        constexpr int V_ = 16 / (int)sizeof(T);                                                   \
         const int per = (a.D + V_ - 1) / V_;                                                      \
         if (a.D <= LN_ROW64) {                                                                    \
             const int ch = (per + 63) / 64;                                                       \
-            if (ch <= 8 / V_) return FN<T, V_, 8 / V_, 64>(a, st);                                \
-            if (ch <= 16 / V_) return FN<T, V_, 16 / V_, 64>(a, st);                              \
-            return FN<T, V_, 24 / V_, 64>(a, st);                                                 \
+            if (ch <= 8 / V_) return FN<T, 8 / V_, 64, AL>(a, st);                                \
+            if (ch <= 16 / V_) return FN<T, 16 / V_, 64, AL>(a, st);                              \
+            return FN<T, 24 / V_, 64, AL>(a, st);                                                 \
         }                                                                                         \
         const int ch = (per + 255) / 256;                                                         \
-        if (ch <= 8 / V_) return FN<T, V_, 8 / V_, 256>(a, st);                                   \
-        if (ch <= 16 / V_) return FN<T, V_, 16 / V_, 256>(a, st);                                 \
-        return FN<T, V_, 32 / V_, 256>(a, st);                                                    \
+        if (ch <= 8 / V_) return FN<T, 8 / V_, 256, AL>(a, st);                                   \
+        if (ch <= 16 / V_) return FN<T, 16 / V_, 256, AL>(a, st);                                 \
+        return FN<T, 32 / V_, 256, AL>(a, st);                                                    \
     } while (0)
 
 // workgroups per batch element of the backward: at most one (eight waves) per CU over all batch elements -- a 257th workgroup would share a CU and
@@ -332,11 +353,11 @@ int layernorm_fwd_impl(const void* x, int64_t ldx, int dtype, const float* gamma
     const bool cols = aligned16(gamma) && aligned16(beta) && (ldg % 4 == 0 || M <= rows_per_batch);
     const bool wide = cols && D % vec == 0 && ldx % vec == 0 && aligned16(x) && aligned16(y);
     if (dtype == 0) {
-        if (wide) LN_PICK(launch_fwd, bf16_t, 8);
-        LN_PICK(launch_fwd, bf16_t, 1);
+        if (wide) LN_PICK(launch_fwd, bf16_t, true);
+        LN_PICK(launch_fwd, bf16_t, false);
     }
-    if (wide) LN_PICK(launch_fwd, float, 4);
-    LN_PICK(launch_fwd, float, 1);
+    if (wide) LN_PICK(launch_fwd, float, true);
+    LN_PICK(launch_fwd, float, false);
 }
 
 int layernorm_bwd_impl(const void* dy, const void* x, int64_t ldx, int dtype, const float* mean, const float* rstd, const float* gamma, int64_t ldg,
@@ -357,11 +378,11 @@ int layernorm_bwd_impl(const void* dy, const void* x, int64_t ldx, int dtype, co
     const bool wide = cols && D % vec == 0 && ldx % vec == 0 && aligned16(x) && aligned16(dy) && aligned16(dx);
     const int rl = [&]() -> int {
         if (dtype == 0) {
-            if (wide) LN_PICK(launch_bwd, bf16_t, 8);
-            LN_PICK(launch_bwd, bf16_t, 1);
+            if (wide) LN_PICK(launch_bwd, bf16_t, true);
+            LN_PICK(launch_bwd, bf16_t, false);
         }
-        if (wide) LN_PICK(launch_bwd, float, 4);
-        LN_PICK(launch_bwd, float, 1);
+        if (wide) LN_PICK(launch_bwd, float, true);
+        LN_PICK(launch_bwd, float, false);
     }();
     if (rl || !a.ws) return rl;
     hipLaunchKernelGGL(ln_bwd_reduce_kernel, dim3((2 * D + 63) / 64, a.nb), dim3(1024), 0, st, ws, D, a.gpb, dgamma, dbeta, (long)ldd, accumulate);
