@@ -57,7 +57,8 @@ struct PAArgs {
     float *lse2, *delta;                               // (H, Tq)
     bf16_t *dQ, *dK, *dV;                              // (Tq, H, 64), (Tk, Hkv, 64)
     float* dist;                                       // [workgroup of the dQ grid][2 R + 1]: sums of dS by distance
-    int nt, nwork;                                     // row tiles per (document, head) of this grid; workgroups that compute
+    int nt, nwork, heads, order;                       // row tiles per (document, head) of this grid; workgroups that compute; heads x parts; longest
+                                                       // documents first
     int splits; float* part;                           // parts of a tile's sweep; dK / dV: their sums [part][dK | dV][Tk][Hkv][64]; forward: their
                                                        // accumulators [part][Tq][H][64], then reference points and sums [part][2][Tq][H]
 };
@@ -88,20 +89,42 @@ __device__ __forceinline__ Doc doc_of(const PAArgs& p, int d) {
     return r;
 }
 
-// Workgroups go to the 8 XCDs round-robin in launch order.  Re-numbered so that an XCD gets a contiguous run of (head, document, tile): the
-// tiles of a (document, head) stream the same K / V through one L2, and with eight or more heads every XCD has all documents (equal work).
+// The document of a given rank by length, longest first (up to 64 documents: a lane each; every wave finds it by itself)
+__device__ __forceinline__ int doc_of_rank(const int* cu, const int* len, int nd, int total, int rank) {
+    const int lane = threadIdx.x & 63;
+    const int n = lane < nd ? span(cu, len, lane, total).n : -1;
+    int r = 0;
+    for (int j = 0; j < nd; ++j) {
+        const int m = __builtin_bit_cast(int, lane_bcast(__builtin_bit_cast(float, n), j));
+        r += (m > n || (m == n && j < lane)) ? 1 : 0;
+    }
+    return uniform_i(__builtin_ctzll(wave_ballot(lane < nd && r == rank)));
+}
+
+// Workgroups go to the 8 XCDs round-robin in launch order.  Re-numbered so that an XCD gets a contiguous run of heads with all their documents and
+// tiles: the tiles of a (document, head) stream the same K / V through one L2, and with heads in eights every XCD has the same work.  Where there are
+// more workgroups than slots the long sweeps go first (cu / len: the axis that a workgroup sweeps, whose length is the workgroup's time) and a
+// document's heads side by side: 11 documents of 97 .. 1056 tokens in a mixed order, forward 91 -> 88 us, dQ 118 -> 116, dK / dV 123 -> 119; six of
+// 1056 and 2112, causal, forward 89 -> 80, dQ 101 -> 96.  A dK / dV sweep in parts is better off as the documents lie (131 against 141 us there).
 struct Work { int h, d, tile, lin; };
-__device__ __forceinline__ Work work_of(const PAArgs& p) {
+__device__ __forceinline__ Work work_of(const PAArgs& p, const int* cu, const int* len, int total) {
     const int q = p.nwork >> 3, r = p.nwork & 7;
-    int lin = (int)blockIdx.x;
-    const int xcd = lin & 7;
-    lin = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (lin >> 3);
+    const int xcd = (int)blockIdx.x & 7, in = (int)blockIdx.x >> 3;
     Work w;
-    w.lin = lin;
-    w.tile = p.nt - 1 - lin % p.nt;          // causal: the long rows first
-    const int hd = lin / p.nt;
-    w.d = hd % p.nd;
-    w.h = hd / p.nd;
+    if (p.order && p.heads % 8 == 0) {       // heads xcd hp .. + hp - 1: document by document, the heads inside
+        const int hp = p.heads >> 3, rest = in / p.nt;
+        w.tile = in % p.nt;
+        w.h = xcd * hp + rest % hp;
+        w.d = rest / hp;
+    } else {
+        const int lin = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + in, hd = lin / p.nt;
+        w.tile = lin % p.nt;
+        w.d = hd % p.nd;
+        w.h = hd / p.nd;
+    }
+    w.tile = p.nt - 1 - w.tile;              // causal: the long rows first
+    if (p.order) w.d = doc_of_rank(cu, len, p.nd, total, w.d);
+    w.lin = (w.h * p.nd + w.d) * p.nt + p.nt - 1 - w.tile;
     return w;
 }
 
@@ -221,7 +244,7 @@ __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
     }
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform_i(tid >> 6);
     const int l31 = lane & 31, hi = lane >> 5;
-    const Work wk = work_of(p);
+    const Work wk = work_of(p, p.cu_k, p.len_k, p.Tk);
     const int h = wk.h / p.splits, part = wk.h % p.splits;
     const Doc D = doc_of(p, wk.d);
     if (wk.tile * 128 >= D.nq) return;
@@ -501,7 +524,7 @@ __global__ __launch_bounds__(256, (BIAS || CAP) ? 2 : 3) void pa_dq_kernel(PAArg
     }
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform_i(tid >> 6);
     const int l31 = lane & 31, hi = lane >> 5;
-    const Work wk = work_of(p);
+    const Work wk = work_of(p, p.cu_k, p.len_k, p.Tk);
     const int h = wk.h;
     const Doc D = doc_of(p, wk.d);
     if (wk.tile * 128 >= D.nq) return;
@@ -720,7 +743,7 @@ __global__ __launch_bounds__(256, 2) void pa_dkv_kernel(PAArgs p) {
     }
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform_i(tid >> 6);
     const int l31 = lane & 31, hi = lane >> 5;
-    Work wk = work_of(p);                          // (key head, document, tile) x part
+    Work wk = work_of(p, p.cu_q, p.len_q, p.Tq);   // (key head, document, tile) x part
     const int part = wk.h % p.splits;
     wk.h /= p.splits;
     const Doc D = doc_of(p, wk.d);
@@ -970,6 +993,8 @@ int plan_grid(PAArgs& a, int longest, int total, int heads, long& grid) {
     grid = work + (a.fill ? ((long)a.nd + 1) * GAP_PARTS : 0);
     if (grid > 0x7fffffffL / 256) return E2K_ERR_SHAPE;
     a.nwork = (int)work;
+    a.heads = heads;
+    a.order = a.nd > 1 && a.nd <= 64 && work > 512;
     return E2K_OK;
 }
 // the same rows in JOIN_ROWS-row tiles
@@ -1093,6 +1118,7 @@ int packed_attn_bwd_impl(const void* dO, int64_t sg, int64_t hg, const void* Q, 
         if (a.splits > 1 && !ws) return E2K_ERR_ARG;
         const int rg = plan_grid(a, max_k, Tk, Hkv * a.splits, grid);
         if (rg) return rg;
+        if (a.splits > 1) a.order = 0;
         if (grid > 0) {
             PA_PICK(run_dkv, a, 0, grid, st);
             E2K_CHECK_LAUNCH();

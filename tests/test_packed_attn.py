@@ -541,3 +541,15 @@ def test_packed_attention_many_documents(dev):
     dq, dk, dv, dtable = ops.packed_attn_bwd(st, c.dout.to(dev))
     for name, t in (('out', out), ('dq', dq), ('dk', dk), ('dv', dv), ('dtable', dtable)):
         held(t, want[name], bound[name], name)
+
+
+def test_packed_attention_longest_first(dev):
+    """more workgroups than slots: documents are taken by length (ties, empty ones, 64 and 65 of them); heads in eights and not"""
+    for lens, H in (([40, 0, 70, 40, 130, 1], 8), ([3] * 63 + [50], 1), ([2] * 64 + [33], 1), ([5, 90, 5], 3)):
+        c = Case(lens, H=H, bias='table', mask='causal')
+        base = run(c, dev)                                   # (no hint: the grid is sized for the total, most of it empty)
+        want, bound = c.exact()
+        for n in want:
+            held(base[n], want[n], bound[n], n)
+        big = run(c, dev, max_q=100 * 128, max_k=100 * 128)
+        assert all(torch.equal(base[n], big[n]) for n in ('out', 'dq', 'dk', 'dv'))
