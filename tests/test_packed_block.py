@@ -217,3 +217,50 @@ def test_recorded_in_a_launch_plan():
     torch.cuda.synchronize()
     assert torch.equal(out, want[0]) and torch.equal(y, want[1])
     L.e2k_plan_free(h)
+
+
+@pytest.mark.gpu
+def test_two_streams_and_next_to_lds_dma_gemms():
+    """the kernels on two streams at once, beside a third that runs LDS-DMA GEMMs: the bits of the same calls alone, every time"""
+    from e2_tts_pytorch_amd import _lib, ops
+    from emu.install import install
+    install(None, False)
+    _lib.get()
+    torch.manual_seed(5)
+    T, H = 1500, 8
+    cu = offsets([700, 96, 704], 'cuda')
+    buckets = ops.rel_buckets(32, 128, device='cuda')
+    table, slopes = torch.randn(32, H, device='cuda'), torch.rand(H, device='cuda')
+    q, k, v, g = (torch.randn(T, H, 64, device='cuda').to(bf16) for _ in range(4))
+    kc, vc = (torch.randn(4, 3000, H, 64, device='cuda').to(bf16) for _ in range(2))
+    n = torch.tensor([3000, 10, 1111, 2222], dtype=torch.int32, device='cuda')
+    x, w = torch.randn(T, 1024, device='cuda').to(bf16), torch.randn(1024, device='cuda')
+
+    def first():
+        out, st = ops.packed_attn_fwd(q, k, v, cu, train=True, table=table, buckets=buckets, softcap=30.)
+        y, m, r = ops.layernorm_fwd(x, w, w)
+        return [out, *ops.packed_attn_bwd(st, g), y, *ops.layernorm_bwd(x, x, m, r, w)]
+
+    def second():
+        out, st = ops.packed_attn_fwd(q, k[:, ::4], v[:, ::4], cu, train=True, causal=True, slopes=slopes)
+        return [out, *ops.packed_attn_bwd(st, g)[:3], ops.packed_attn_fwd(q[:40], k, v, cu.new_tensor([0, 40]), cu.new_tensor([0, T])),
+                ops.attn_decode(q[:4], kc, vc, n, slopes=slopes)]
+
+    want = first(), second()
+    a, b = torch.randn(4096, 1024, device='cuda').to(bf16), torch.randn(4096, 1024, device='cuda').to(bf16)
+    torch.cuda.synchronize()
+    s1, s2, s3 = (torch.cuda.Stream() for _ in range(3))
+    bad = 0
+    for _ in range(30):
+        got = [[], []]
+        for _ in range(3):
+            with torch.cuda.stream(s3):
+                for _ in range(6):
+                    ops.gemm_nt(a, b)
+            for s, f, o in ((s1, first, got[0]), (s2, second, got[1])):
+                with torch.cuda.stream(s):
+                    o.append(f())
+        torch.cuda.synchronize()
+        for res, ref in zip(got, want):
+            bad += sum(not torch.equal(t, u) for one in res for t, u in zip(one, ref))
+    assert bad == 0, bad
