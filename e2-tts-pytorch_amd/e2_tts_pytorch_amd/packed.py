@@ -44,7 +44,9 @@ class _PackedAttnFn(Function):
 def packed_attention(q, k, v, cu_q, cu_k=None, *, len_q=None, len_k=None, prefix=None, max_q=0, max_k=0, causal=False, scale=None, softcap=0., slopes=None,
                      bias=None):
     """ops.packed_attn_fwd with gradients for q, k, v and the bias: q (Tq,H,64), k / v (Tk,Hkv,64) bf16, documents at the offsets cu_q / cu_k; `bias` a
-    RelativePositionBias.  `slopes` are constants: a tensor that wants a gradient is refused.  -> (Tq,H,64) bf16"""
+    RelativePositionBias.  `slopes` are constants: a tensor that wants a gradient is refused.  Into a HIP graph capture a training pass with
+    torch.autograd.grad (or the ops calls): accumulating into .grad of leaves that an eager graph still holds on another stream cannot be captured.
+    -> (Tq,H,64) bf16"""
     if slopes is not None and slopes.requires_grad:
         raise ops.E2KError('packed_attention: slopes get no gradient; pass slopes.detach(), or learn a RelativePositionBias')
     table, buckets = (None, None) if bias is None else (bias.weight, bias.buckets)

@@ -264,3 +264,45 @@ def test_two_streams_and_next_to_lds_dma_gemms():
         for res, ref in zip(got, want):
             bad += sum(not torch.equal(t, u) for one in res for t, u in zip(one, ref))
     assert bad == 0, bad
+
+
+@pytest.mark.gpu
+def test_autograd_captured():
+    """forward and torch.autograd.grad of the block in one captured graph, replayed on changed inputs"""
+    from e2_tts_pytorch_amd import _lib
+    from emu.install import install
+    install(None, False)
+    _lib.get()
+    torch.manual_seed(6)
+    lens = [150, 70]
+    cu = offsets(lens, 'cuda')
+    blk = Block(heads=4, kv_heads=2).cuda()
+    ps = list(blk.parameters())
+    x = torch.randn(sum(lens), 128, device='cuda').to(bf16).requires_grad_()
+    dy = torch.randn(sum(lens), 128, device='cuda').to(bf16)
+
+    def f():
+        y = blk(x, cu, max_q=150, causal=True)
+        return [y.detach(), *torch.autograd.grad(y, [x] + ps, dy)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            f()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        res = f()
+    for i in range(3):
+        with torch.no_grad():
+            x.normal_()
+            dy.normal_()
+        want = f()
+        torch.cuda.synchronize()
+        gr.replay()
+        torch.cuda.synchronize()
+        # (the projections' library products may take another kernel inside the graph: bf16 roundings of the same values)
+        for a, b in zip(res, want):
+            assert (a.float() - b.float()).norm() <= 0.02 * b.float().norm(), i
