@@ -24,7 +24,8 @@
 // The backward works with small differences p (dO.v - dO.o), and the table's gradient is a sum of them over every pair at a distance, in fp32: an
 // o that is good to bf16 only (probabilities rounded before the second product, output rounded after it) shows in the gradients of q and k (2.9e-3
 // off the exact ones instead of 2.4e-3) and in the third digit of the table's.  A training forward therefore carries the probabilities as two bf16
-// terms through the second product and keeps what rounding cut off the output (o_lo): dO.o is then good to 2^-16 of its terms.
+// terms through the second product and keeps what rounding cut off the output (o_lo, bf16); with a table as three terms and o_lo in fp32 (its
+// gradient is then 6e-7 off, as in plain fp32, instead of 3e-6; 89 -> 101 us on 8397 tokens of 11 documents, 16 heads).
 //
 // Sums are taken in a fixed order throughout: no atomics, the same bits every time.
 #include "e2k_device.h"
@@ -53,7 +54,7 @@ struct PAArgs {
     float scale, cap;
     int causal, fill;
     const float *slopes, *table; const int* buckets; int nbuckets, R;
-    bf16_t *O, *Olo;                                   // O strided; Olo (Tq, H, 64)
+    bf16_t* O; void* Olo;                              // O strided; Olo (Tq, H, 64): fp32 with a table, else bf16
     float *lse2, *delta;                               // (H, Tq)
     bf16_t *dQ, *dK, *dV;                              // (Tq, H, 64), (Tk, Hkv, 64)
     float* dist;                                       // [workgroup of the dQ grid][2 R + 1]: sums of dS by distance
@@ -234,7 +235,7 @@ struct Stager {
 // while one is computed: with one, the copies' latency of about 1 us set the pace; one raw barrier a tile), three workgroups a CU.
 // Bound by the vector ALU (88 % of its busy clocks on long rows): 16417 tokens x 16 heads, linear bias, cap: 1.96 ms, 562 TFLOP/s; 8 x 1056 tokens x
 // 16 heads, no bias: 59 us, 618 TFLOP/s (83 with the training form's second term).
-// TRAIN: log-sum-exps, two-term probabilities, o_lo
+// TRAIN: log-sum-exps, probabilities in two terms (with a table three), o_lo
 template <int BIAS, bool CAP, bool TRAIN>
 __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
     __shared__ __attribute__((aligned(16))) unsigned char smem[NST * STAGE];
@@ -289,9 +290,9 @@ __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
         if (kt0 < nt) fetch(kt0, smem);
         if (kt0 + 1 < nt) fetch(kt0 + 1, smem + STAGE);
         const int qp = q0 + D.off;
-        // probabilities (arguments of exp2 in x) packed, in training with what packing cut off as a second term, and the row's sum with them (of the
-        // packed ones: its error is theirs over the square root of their number; of the unrounded ones where fp32 results depend on it)
-        auto probs = [&](float (&x)[16], bf16x8 (&pf)[2], bf16x8 (&pl)[2], float& la, float& lb) __attribute__((always_inline)) {
+        // probabilities (arguments of exp2 in x, replaced) packed, and the row's sum with them (of the packed ones: its error is theirs over the square
+        // root of their number; of the unrounded ones where fp32 results depend on it)
+        auto probs = [&](float (&x)[16], bf16x8 (&pf)[2], float& la, float& lb) __attribute__((always_inline)) {
             la = l0;
             lb = l1;
 #pragma unroll
@@ -309,16 +310,6 @@ __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
                 for (int i = 0; i < 4; ++i) {
                     la = add_bf16_pair(__builtin_bit_cast(u32x4, pf[0])[i], la);
                     lb = add_bf16_pair(__builtin_bit_cast(u32x4, pf[1])[i], lb);
-                }
-            }
-            if (TRAIN) {
-#pragma unroll
-                for (int s2 = 0; s2 < 2; ++s2) {
-                    float w[8];
-                    unpack8(__builtin_bit_cast(u32x4, pf[s2]), w);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) w[e] = x[8 * s2 + e] - w[e];
-                    pl[s2] = pack8f(w);
                 }
             }
         };
@@ -342,21 +333,19 @@ __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
                 sched_fence();
                 tr_frags<S + 8192 + kb * 4096>(vf, tra);
                 sched_fence();
-                float la, lb;
-                bf16x8 pf[2], pl[2];
+                float la, lb, x[16];
+                bf16x8 pf[2];
                 const int rel = kk + 8 * hi - (qp + l31), lo = kk - qp;
                 bool done = false;
                 if (kk + 32 <= lim_lo) {                      // every query of the wave sees all of the block
-                    float x[16];
                     f32x16 z = s;
                     const float mo = m - sc.offset(rel, lo);
                     sc.args(z, x, rel, lo, [&](int) { return mo; });
-                    probs(x, pf, pl, la, lb);
+                    probs(x, pf, la, lb);
                     done = wave_all(la + lb < L_MAX);
                 }
                 if (!done) {                                  // a masked block, or a row whose sum outgrew its reference point
                     cold_path();
-                    float x[16];
                     pin_vgpr(s);                                          // (its arithmetic is not shared with the path above: that would keep 32 registers alive)
                     const float c = sc.offset(rel, lo);
                     sc.args(s, x, rel, lo, [](int) { return 0.f; });
@@ -376,7 +365,7 @@ __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
                     m = mn;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) x[r] -= mn - c;
-                    probs(x, pf, pl, la, lb);
+                    probs(x, pf, la, lb);
                 }
                 l0 = la;
                 l1 = lb;
@@ -384,12 +373,19 @@ __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
                 for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
                     for (int db = 0; db < 2; ++db) o[db] = mfma32(vf[s2][db], pf[s2], o[db]);
-                if (TRAIN) {
+                // what packing cut off, as a second (third) term
 #pragma unroll
-                    for (int s2 = 0; s2 < 2; ++s2)
+                for (int term = 1; term < (FINE ? 3 : TRAIN ? 2 : 1); ++term)
 #pragma unroll
-                        for (int db = 0; db < 2; ++db) o[db] = mfma32(vf[s2][db], pl[s2], o[db]);
-                }
+                    for (int s2 = 0; s2 < 2; ++s2) {
+                        float w[8];
+                        unpack8(__builtin_bit_cast(u32x4, pf[s2]), w);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[8 * s2 + e] -= w[e];
+                        pf[s2] = pack8f(x + 8 * s2);
+#pragma unroll
+                        for (int db = 0; db < 2; ++db) o[db] = mfma32(vf[s2][db], pf[s2], o[db]);
+                    }
             };
             block(Int<0>{});
             block(Int<1>{});
@@ -421,7 +417,7 @@ __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
             const int row = D.q0 + (qin ? q : 0);
             if (TRAIN && qin && hi == 0) p.lse2[(long)h * p.Tq + row] = l == 0.f ? LSE_EMPTY : m + log2f(l);
             bf16_t* orow = p.O + (long)row * p.so + (long)h * p.ho;
-            bf16_t* lrow = TRAIN ? p.Olo + ((long)row * p.H + h) * DH : nullptr;
+            const long lrow = ((long)row * p.H + h) * DH;
             store_rows32(o, hi, qin, [&](int db, int g, int hi_, bool ok, const float* a, const float* b) __attribute__((always_inline)) {
                 float v[8];
 #pragma unroll
@@ -433,6 +429,13 @@ __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
                     unpack4(y, w + 4);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) lo[e] = v[e] - w[e];
+                    if (FINE) {
+                        float* lf = (float*)p.Olo + lrow + 32 * db + 8 * g + 4 * hi_;
+                        if (ok) {
+                            st<f32x4>(lf, f32x4{lo[0], lo[1], lo[2], lo[3]});
+                            st<f32x4>(lf + 8, f32x4{lo[4], lo[5], lo[6], lo[7]});
+                        }
+                    }
                     xl = pack4(lo);
                     yl = pack4(lo + 4);
                     swap_pair(xl, yl);
@@ -441,7 +444,7 @@ __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
                 const int col = 32 * db + 8 * (g + hi_);
                 if (ok) {
                     st<u32x4>(orow + col, u32x4{x[0], x[1], y[0], y[1]});
-                    if (TRAIN) st<u32x4>(lrow + col, u32x4{xl[0], xl[1], yl[0], yl[1]});
+                    if (TRAIN && !FINE) st<u32x4>((bf16_t*)p.Olo + lrow + col, u32x4{xl[0], xl[1], yl[0], yl[1]});
                 }
             });
         }
@@ -569,12 +572,19 @@ __global__ __launch_bounds__(256, (BIAS || CAP) ? 2 : 3) void pa_dq_kernel(PAArg
         float dl = 0.f;
         {
             const bf16_t* orow = p.O + (long)row * p.so + (long)h * p.ho + hi * 8;
-            const bf16_t* lrow = p.Olo + ((long)row * p.H + h) * DH + hi * 8;
+            const long lrow = ((long)row * p.H + h) * DH + hi * 8;
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) {
                 float a[8], b[8], g[8];
                 unpack8(ld<u32x4>(orow + ks * 16), a);
-                unpack8(ld<u32x4>(lrow + ks * 16), b);
+                if (BIAS == 2) {
+                    const float* lf = (const float*)p.Olo + lrow + ks * 16;
+                    const f32x4 u = ld<f32x4>(lf), w = ld<f32x4>(lf + 4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { b[e] = u[e]; b[4 + e] = w[e]; }
+                } else {
+                    unpack8(ld<u32x4>((const bf16_t*)p.Olo + lrow + ks * 16), b);
+                }
                 unpack8(__builtin_bit_cast(u32x4, dof[ks]), g);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) dl = fmaf(g[e], a[e] + b[e], dl);
@@ -1051,7 +1061,7 @@ int packed_attn_fwd_impl(const void* Q, int64_t sq, int64_t hq, const void* K, i
                          int fill_gaps, void* stream) {
     PAArgs a = common(Q, sq, hq, K, sk, hk, V, sv, hv, cu_q, cu_k, len_q, len_k, prefix, nd, Tq, Tk, H, Hkv, causal, scale, softcap, slopes, table,
                       buckets, nbuckets, reach);
-    a.O = (bf16_t*)O; a.so = so; a.ho = ho; a.Olo = (bf16_t*)Olo; a.lse2 = lse2; a.fill = fill_gaps;
+    a.O = (bf16_t*)O; a.so = so; a.ho = ho; a.Olo = (void*)Olo; a.lse2 = lse2; a.fill = fill_gaps;
     if (Tq == 0) return E2K_OK;
     const int rc = check(a);
     if (rc) return rc;
@@ -1083,7 +1093,7 @@ int packed_attn_bwd_impl(const void* dO, int64_t sg, int64_t hg, const void* Q, 
                          int fill_gaps, void* stream) {
     PAArgs a = common(Q, sq, hq, K, sk, hk, V, sv, hv, cu_q, cu_k, len_q, len_k, prefix, nd, Tq, Tk, H, Hkv, causal, scale, softcap, slopes, table,
                       buckets, nbuckets, reach);
-    a.dO = (const bf16_t*)dO; a.sg = sg; a.hg = hg; a.O = (bf16_t*)O; a.so = so; a.ho = ho; a.Olo = (bf16_t*)Olo; a.lse2 = (float*)lse2; a.delta = delta;
+    a.dO = (const bf16_t*)dO; a.sg = sg; a.hg = hg; a.O = (bf16_t*)O; a.so = so; a.ho = ho; a.Olo = (void*)Olo; a.lse2 = (float*)lse2; a.delta = delta;
     a.dQ = (bf16_t*)dQ; a.dK = (bf16_t*)dK; a.dV = (bf16_t*)dV; a.dist = ws; a.fill = fill_gaps;
     hipStream_t st = (hipStream_t)stream;
     long grid;

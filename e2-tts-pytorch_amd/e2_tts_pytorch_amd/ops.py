@@ -1157,7 +1157,7 @@ def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, len_q=None, len_k=None, prefix=
         raise E2KError('packed attention: out must be a (Tq, H, 64) bf16 tensor like q with 16-byte rows that do not overlap')
     lo = lse2 = ws = None
     if train:
-        lo = torch.empty((Tq, H, 64), dtype=bf16, device=dev)
+        lo = torch.empty((Tq, H, 64), dtype=bf16 if table is None else f32, device=dev)
         lse2 = torch.empty((H, Tq), dtype=f32, device=dev)
     else:
         n = _lib.get().e2k_query_packed_attn_fwd_ws_floats(Tq, Tk, H, int(max_k))

@@ -356,7 +356,7 @@ int e2k_freq_attn_bwd(const void* dout, const void* qkv, int64_t ld, const void*
  * (positions; slopes fp32 (H); table fp32 (nbuckets, H); buckets int32 (2 reach + 1) by key minus query distance, clamped at +-reach <= 512; one of
  * slopes / table or neither), softmax over the visible keys, O = P V; a row that sees nothing is 0.  A bias of -1e30 or less hides its keys.
  * O (Tq, H, 64) strided; rows that no document covers are zeroed with fill_gaps = 1, left alone with 0.  For the backward: Olo
- * (Tq, H, 64) contiguous (what rounding to bf16 cut off O) and lse2 (H, Tq) fp32 (log2 domain), both or neither.
+ * (Tq, H, 64) contiguous, fp32 with a table and bf16 without (what rounding to bf16 cut off O), and lse2 (H, Tq) fp32 (log2 domain), both or neither.
  * max_q (max_k): the longest document, a sizing hint -- longer ones are computed all the same; 0 = unknown.
  * ws: e2k_query_packed_attn_fwd_ws_floats floats, 16-byte aligned, without Olo (0, or with Olo: NULL will do). */
 int64_t e2k_query_packed_attn_fwd_ws_floats(int Tq, int Tk, int H, int max_k);

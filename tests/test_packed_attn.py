@@ -120,7 +120,7 @@ class Case:
                 r['dv'][B, h // G] += p.t() @ dO
                 b['dv'][B, h // G] += (p * (HALF + ep)).t() @ dO.abs()
                 if self.table is not None:
-                    # the table's gradient: dO.o is good to 2^-16 of its terms (two-term probabilities and output); fp32 sums over the document's pairs
+                    # the table's gradient: dO.o is good to 2^-16 of its terms or better (three-term probabilities, fp32 remainder of the output); fp32 sums over the document's pairs
                     edl = ((dO.abs() * ((p * (2. ** -16 + ep)) @ V.abs() + 2. ** -16 * o.abs())).sum(1, keepdim=True))
                     eds = p * (ep * (dP - dl).abs() + 64 * U * (mdP + dl.abs()) + edl) + 64 * U * ds.abs()
                     where = self.map.long()[rel.clamp(-self.reach, self.reach) + self.reach]
