@@ -290,8 +290,9 @@ __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
         if (kt0 < nt) fetch(kt0, smem);
         if (kt0 + 1 < nt) fetch(kt0 + 1, smem + STAGE);
         const int qp = q0 + D.off;
-        // probabilities (arguments of exp2 in x, replaced) packed, and the row's sum with them (of the packed ones: its error is theirs over the square
-        // root of their number; of the unrounded ones where fp32 results depend on it)
+        // probabilities (arguments of exp2 in x, replaced) packed, and the row's sum with them: of the packed ones in inference, whose second product has
+        // no more than them (what rounds a dominating one up rounds the sum up too); of the unrounded ones in training, whose second product has them in
+        // two or three terms (with the packed ones' sum a peaked row's output and log-sum-exp were up to 2^-8 off)
         auto probs = [&](float (&x)[16], bf16x8 (&pf)[2], float& la, float& lb) __attribute__((always_inline)) {
             la = l0;
             lb = l1;
@@ -299,7 +300,7 @@ __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
             for (int r = 0; r < 16; ++r) x[r] = fast_exp2(x[r]);
             pf[0] = pack8f(x);
             pf[1] = pack8f(x + 8);
-            if (FINE) {
+            if (TRAIN) {
 #pragma unroll
                 for (int r = 0; r < 16; r += 2) {
                     la += x[r];
