@@ -8,6 +8,7 @@ import contextlib
 
 import ctypes
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -93,6 +94,47 @@ class _on_device:
         if self.guard is not None:
             self.guard.__exit__(*exc)
         return False
+
+
+def _row_dims(t):
+    """(size, stride) of the dimensions that t's rows (last dimension, contiguous) are laid out by, largest stride first; None where rows overlap or
+    are not nested (every stride as long as what lies inside it)"""
+    dims = sorted(((n, st) for n, st in zip(t.shape[:-1], t.stride()) if n > 1), key=lambda d: -d[1])
+    inner = t.shape[-1]
+    for n, st in reversed(dims):
+        if st < inner:
+            return None
+        inner += (n - 1) * st
+    return dims
+
+
+def _rows_meet(a, b):
+    """whether two tensors of equally wide rows and one type share an element.  a's rows must not overlap (_row_dims); where b's are not nested, whether the
+    address ranges meet"""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    size = a.element_size()
+    at = (a.data_ptr() - b.data_ptr()) // size
+
+    def extent(t):
+        return sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1
+    if at >= extent(b) or at + extent(a) <= 0:
+        return False
+    outer, inner = _row_dims(a), _row_dims(b)
+    if inner is None:
+        return True
+    width = a.shape[-1]
+    # rows of a, as offsets from b's first; a dimension with the stride of b's outermost (tokens of one buffer) needs no list: b's index moves along
+    starts, back = np.array([at]), 0
+    for n, st in outer:
+        if inner and st == inner[0][1]:
+            back = n - 1
+        else:
+            starts = (starts[:, None] + st * np.arange(n)).ravel()
+    for n, st in inner:
+        starts = np.concatenate([starts - np.clip((starts + edge) // st, -back, n - 1) * st for edge in (0, width - 1)])
+        back = 0
+    return bool((np.abs(starts) < width).any())
 
 
 def lib():
@@ -1063,6 +1105,14 @@ def _heads64(t, what):
     return t
 
 
+def _apart(out, q, k, v, what, in_place):
+    """refuses an output that shares memory with what other workgroups still read.  in_place: it may be q itself (a row of q is read by the workgroups
+    that its output row waits for, and by no other)"""
+    same = in_place and out.data_ptr() == q.data_ptr() and all(n == 1 or s == t for n, s, t in zip(q.shape, q.stride(), out.stride()))
+    if (not same and _rows_meet(out, q)) or _rows_meet(out, k) or _rows_meet(out, v):
+        raise E2KError(f'{what}: out shares memory with ' + ('k or v, or with q without being it' if in_place else 'q, k or v'))
+
+
 def _offsets(cu, what, device, n=None):
     if cu.dtype != torch.int32 or cu.dim() != 1 or not cu.is_contiguous() or cu.device != device or (cu.numel() != n if n is not None else cu.numel() < 1):
         raise E2KError(f'packed attention: {what} must be contiguous int32 on the device of q' + (f', {n} of them' if n is not None else ''))
@@ -1125,7 +1175,7 @@ def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, len_q=None, len_k=None, prefix=
     prefix[d] keys.  softcap > 0: scores capped to softcap * tanh(score / softcap).  slopes (H,) fp32: bias -slope * distance; or table (buckets,H) fp32
     with buckets (2 reach + 1,) int32: learned bias by key - query distance (rel_buckets).  max_q / max_k: longest document, a sizing hint.
     -> out (Tq,H,64) bf16, with train=True (out, state for packed_attn_bwd).  Rows that no document covers: zero, or left alone in an `out` given by the
-    caller.  Offsets have to be non-decreasing.  NaN / inf outside a document never reaches it; inside, a NaN / inf key or value may reach any query of
+    caller; `out` must not share memory with q, k and v (without train=True it may be q itself).  Offsets have to be non-decreasing.  NaN / inf outside a document never reaches it; inside, a NaN / inf key or value may reach any query of
     its document.  Biases of -1e30 or less hide their keys."""
     _chk(q, k, v, cu_q, cu_k, len_q, len_k, prefix, slopes, table, buckets, out)
     q, k, v = _heads64(q, 'q'), _heads64(k, 'k'), _heads64(v, 'v')
@@ -1152,9 +1202,11 @@ def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, len_q=None, len_k=None, prefix=
     fill = out is None
     if fill:
         out = torch.empty((Tq, H, 64), dtype=bf16, device=dev)
-    elif out.shape != q.shape or out.dtype != bf16 or out.device != dev or out.stride(2) != 1 or out.stride(0) % 8 or out.stride(1) % 8 or out.data_ptr() % 16 \
-            or out.stride(0) >= 1 << 23 or not (out.stride(1) >= 64 and out.stride(0) >= H * 64 or (out.stride(0) >= 64 and out.stride(1) >= Tq * out.stride(0))):
-        raise E2KError('packed attention: out must be a (Tq, H, 64) bf16 tensor like q with 16-byte rows that do not overlap')
+    else:
+        if out.shape != q.shape or out.dtype != bf16 or out.device != dev or out.stride(2) != 1 or out.stride(0) % 8 or out.stride(1) % 8 or out.data_ptr() % 16 \
+                or out.stride(0) >= 1 << 23 or _row_dims(out) is None:
+            raise E2KError('packed attention: out must be a (Tq, H, 64) bf16 tensor like q with 16-byte rows that do not overlap')
+        _apart(out, q, k, v, 'packed attention', not train)
     lo = lse2 = ws = None
     if train:
         lo = torch.empty((Tq, H, 64), dtype=bf16 if table is None else f32, device=dev)
@@ -1217,7 +1269,8 @@ def packed_attn_bwd(st, dout, dtable=None, need_table=True):
 def attn_decode(q, k_cache, v_cache, lens, *, scale=None, softcap=0., slopes=None, table=None, buckets=None, out=None):
     """One query token per sequence over its cached keys: q (B,H,64), k_cache / v_cache (B,capacity,Hkv,64) bf16 (any strides with 16-byte rows: head-major
     caches as transposed views, slices of larger ones), lens (B,) int32 on the device: sequence b has lens[b] keys (cut off at the capacity), the query
-    is the last of them.  Scores as in packed_attn_fwd with causal=True.  -> out (B,H,64) bf16; zero where lens is 0.  Cache rows past lens are not read"""
+    is the last of them.  Scores as in packed_attn_fwd with causal=True.  -> out (B,H,64) bf16; zero where lens is 0.  Cache rows past lens are not read.
+    `out` may be q, and must not share memory with the caches otherwise"""
     _chk(q, k_cache, v_cache, lens, slopes, table, buckets, out)
     if q.dim() != 3 or q.shape[2] != 64 or q.dtype != bf16:
         raise E2KError(f'attn_decode: q must be (sequences, heads, 64) bf16, got {q.dtype} {tuple(q.shape)}')
@@ -1237,8 +1290,10 @@ def attn_decode(q, k_cache, v_cache, lens, *, scale=None, softcap=0., slopes=Non
     scale, softcap, nb, reach = _score_args(H, dev, scale, softcap, slopes, table, buckets, 'attn_decode')
     if out is None:
         out = torch.empty((B, H, 64), dtype=bf16, device=dev)
-    elif out.shape != (B, H, 64) or out.dtype != bf16 or out.stride(2) != 1 or out.device != dev or (B > 1 and out.stride(0) < 64) or (H > 1 and out.stride(1) < 64):
-        raise E2KError('attn_decode: out must be (sequences, heads, 64) bf16 like q, with contiguous rows that do not overlap')
+    else:
+        if out.shape != (B, H, 64) or out.dtype != bf16 or out.stride(2) != 1 or out.device != dev or _row_dims(out) is None:
+            raise E2KError('attn_decode: out must be (sequences, heads, 64) bf16 like q, with contiguous rows that do not overlap')
+        _apart(out, q, k_cache, v_cache, 'attn_decode', True)
     L = _lib.get()
     n = L.e2k_query_attn_decode_ws_floats(B, cap, H, Hkv)
     ws = torch.empty(n, dtype=f32, device=dev) if n else None

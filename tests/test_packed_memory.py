@@ -1,0 +1,84 @@
+"""Which memory the packed operators may share, and which tensors they take as they lie: outputs that overlap an input, tensors off the 16-byte grid, calls
+with nothing on one side."""
+import random
+
+import pytest
+import torch
+
+from test_packed_attn import Case, held, offsets
+
+bf16, f32, f64 = torch.bfloat16, torch.float32, torch.float64
+
+
+def test_rows_meet():
+    """against the elements' addresses, for random views of one buffer"""
+    from e2_tts_pytorch_amd import ops
+    rng = random.Random(0)
+    seen = {True: 0, False: 0}
+    for _ in range(3000):
+        views = []
+        for dims in (2, rng.choice([2, 3])):
+            n = [rng.randint(1, 4) for _ in range(dims)]
+            st, inner = [], 4                                # nested strides, in any order of the dimensions
+            for m in n:
+                st.append(inner + rng.choice([0, 0, 1, 4, 8]) if rng.random() < 0.7 else 4 * rng.randint(1, 12))
+                inner = max(inner, (m - 1) * st[-1] + inner)
+            order = rng.sample(range(dims), dims)
+            views.append(([n[i] for i in order], [st[i] for i in order], rng.randint(0, 60)))
+        buf = torch.zeros(4000)
+        a, b = (buf.as_strided(n + [4], st + [1], at) for n, st, at in views)
+        if ops._row_dims(a) is None or ops._row_dims(b) is None:
+            continue
+
+        def cells(t):
+            idx = torch.zeros(4000)
+            idx.as_strided(t.shape, t.stride(), t.storage_offset()).fill_(1.)
+            return idx
+        want = bool((cells(a) * cells(b)).any())
+        seen[want] += 1
+        assert ops._rows_meet(a, b) == want, views
+    assert min(seen.values()) > 300
+    assert ops._row_dims(torch.zeros(1, 4).expand(3, 4)) is None and not ops._rows_meet(torch.zeros(3, 4), torch.zeros(3, 4))
+
+
+def test_packed_attention_out_beside_its_inputs(dev):
+    """an `out` in the buffer of q, k and v, and q itself as `out`: the same bits as an `out` of its own"""
+    from e2_tts_pytorch_amd import ops
+    for kw in (dict(ql=[37, 40], H=2), dict(ql=[9, 4], kl=[700, 30], H=2)):                # (the second in parts)
+        c = Case(**kw)
+        a, kw = c.args(dev)
+        T, S = c.q.shape[0], c.k.shape[0]
+        want = ops.packed_attn_fwd(*a, **kw)
+        buf = torch.zeros(max(T, S), 4, 2, 64, dtype=bf16, device=dev)
+        q, k, v, out = buf[:T, 0], buf[:S, 1], buf[:S, 2], buf[:T, 3]
+        q.copy_(a[0]), k.copy_(a[1]), v.copy_(a[2])
+        assert torch.equal(ops.packed_attn_fwd(q, k, v, *a[3:], out=out, **kw), want)
+        assert torch.equal(ops.packed_attn_fwd(q, k, v, *a[3:], out=q, **kw), want) and torch.equal(q, want)
+    c = Case([1] * 3, kl=[40] * 3, H=8, Hkv=2, mask='causal')
+    q, k, v = c.q.to(dev), c.k.view(3, 40, 2, 64).to(dev), c.v.view(3, 40, 2, 64).to(dev)
+    n = torch.tensor([40, 7, 33], dtype=torch.int32, device=dev)
+    want = ops.attn_decode(q, k, v, n)
+    assert torch.equal(ops.attn_decode(q, k, v, n, out=q), want) and torch.equal(q, want)
+
+
+def test_overlapping_outputs_are_refused(emu):
+    from e2_tts_pytorch_amd import ops
+    z = lambda *s: torch.zeros(*s, dtype=bf16)  # noqa: E731
+    cu = offsets([10, 6])
+    f = ops.packed_attn_fwd
+    buf, wide = z(17, 3, 2, 64), z(16, 4, 64)
+    q, k, v = buf[:16].unbind(1)
+    two = z(2, 16, 2, 64)
+    bad = [lambda: f(q, k, v, cu, out=k), lambda: f(q, k, v, cu, out=v), lambda: f(q, k, v, cu, out=buf[1:, 0]), lambda: f(q, k, v, cu, out=buf[1:, 1]),
+           lambda: f(q, k, v, cu, out=q, train=True), lambda: f(wide[:, :2], k, v, cu, out=wide[:, 1:3]), lambda: f(q, wide[:, :2], v, cu, out=wide[:, 1:3]),
+           lambda: f(two[0].reshape(2, 16, 64).transpose(0, 1), k, v, cu, out=two[0]), lambda: f(q, k, v, cu, out=z(40, 64).as_strided((16, 2, 64), (128, 128, 1))),
+           lambda: f(q, k, v, cu, out=z(40, 64).as_strided((16, 2, 64), (128, 64, 1), 64).as_strided((16, 2, 64), (128, 192, 1)))]
+    kc, L = z(3, 8, 2, 64), torch.ones(3, dtype=torch.int32)
+    d, qs = ops.attn_decode, z(4, 2, 64)
+    bad += [lambda: d(qs[:3], kc, kc.clone(), L, out=kc[:, 3]), lambda: d(qs[:3], kc.clone(), kc, L, out=kc[:, 7]), lambda: d(qs[:3], kc, kc, L, out=qs[1:]),
+            lambda: d(qs[:3], kc, kc, L, out=z(9, 64).as_strided((3, 2, 64), (64, 64, 1)))]
+    for i, g in enumerate(bad):
+        with pytest.raises(ops.E2KError):
+            g()
+            print('not refused:', i)
+    assert d(qs[:3], kc, kc, L, out=z(3, 3, 64)[:, 1:]).shape == (3, 2, 64)
