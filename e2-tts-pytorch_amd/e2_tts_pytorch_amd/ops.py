@@ -1101,7 +1101,7 @@ def _heads64(t, what):
         raise E2KError(f'packed attention: {what} must be (tokens, heads, 64) bf16, got {t.dtype} {tuple(t.shape)}')
     s0, s1, s2 = t.stride()
     if s2 != 1 or s0 % 8 or s1 % 8 or s0 >= 1 << 23 or t.data_ptr() % 16:
-        t = t.contiguous()
+        t = t.clone(memory_format=torch.contiguous_format)          # (contiguous() hands back a contiguous tensor wherever it starts)
     return t
 
 
@@ -1286,7 +1286,7 @@ def attn_decode(q, k_cache, v_cache, lens, *, scale=None, softcap=0., slopes=Non
     if lens.dtype != torch.int32 or lens.shape != (B,) or not lens.is_contiguous() or lens.device != dev:
         raise E2KError(f'attn_decode: lens must be contiguous int32 ({B},) on the device of q')
     if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
-        q = q.contiguous()
+        q = q.clone(memory_format=torch.contiguous_format)
     scale, softcap, nb, reach = _score_args(H, dev, scale, softcap, slopes, table, buckets, 'attn_decode')
     if out is None:
         out = torch.empty((B, H, 64), dtype=bf16, device=dev)

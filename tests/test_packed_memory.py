@@ -82,3 +82,28 @@ def test_overlapping_outputs_are_refused(emu):
             g()
             print('not refused:', i)
     assert d(qs[:3], kc, kc, L, out=z(3, 3, 64)[:, 1:]).shape == (3, 2, 64)
+
+def test_contiguous_but_misaligned_tensors_are_copied(dev):
+    """q, k, v, dout and a decode q at an odd element of a flat buffer; a single row with a stride that no row of it uses"""
+    from e2_tts_pytorch_amd import ops
+
+    def moved(t):
+        flat = torch.zeros(t.numel() + 1, dtype=t.dtype, device=t.device)
+        flat[1:] = t.flatten()
+        return flat[1:].view(t.shape)
+    c = Case([37, 20], H=2, bias='alibi')
+    a, kw = c.args(dev)
+    out, st = ops.packed_attn_fwd(*a, train=True, **kw)
+    want = [out, *ops.packed_attn_bwd(st, c.dout.to(dev))[:3]]
+    out, st = ops.packed_attn_fwd(*(moved(t) for t in a[:3]), *a[3:], train=True, **kw)
+    got = [out, *ops.packed_attn_bwd(st, moved(c.dout.to(dev)))[:3]]
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    assert torch.equal(ops.packed_attn_fwd(*(moved(t) for t in a[:3]), *a[3:], **kw), ops.packed_attn_fwd(*a, **kw))
+    q, k, v = a[0][:2].contiguous(), a[1][:40].view(2, 20, 2, 64), a[2][:40].view(2, 20, 2, 64)
+    n = torch.tensor([20, 7], dtype=torch.int32, device=dev)
+    assert torch.equal(ops.attn_decode(moved(q), k, v, n), ops.attn_decode(q, k, v, n))
+    one = torch.zeros(2 * 64 + 64, dtype=bf16, device=dev).as_strided((1, 2, 64), (131, 64, 1))
+    one.copy_(q[:1])
+    cu = offsets([1], dev)
+    assert torch.equal(ops.packed_attn_fwd(one, one, one, cu), ops.packed_attn_fwd(q[:1], q[:1], q[:1], cu))
+    assert torch.equal(ops.attn_decode(one, k[:1], v[:1], n[:1]), ops.attn_decode(q[:1], k[:1], v[:1], n[:1]))
