@@ -7,11 +7,19 @@ from __future__ import annotations
 
 import torch
 from torch import nn
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 
 from . import ops
 
 __all__ = ['packed_attention', 'attn_decode', 'RelativePositionBias', 'LayerNorm', 'layer_norm']
+
+
+def _no_tangents(what, *ts):
+    """refuses forward-mode duals, which a call that goes past autograd (or hides an input in its options) would drop without a word"""
+    if forward_ad._current_level < 0:             # (no dual level is open: nothing to unpack)
+        return
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise ops.E2KError(f'{what}: no forward-mode gradients')
 
 
 class _PackedAttnFn(Function):
@@ -50,6 +58,7 @@ def packed_attention(q, k, v, cu_q, cu_k=None, *, len_q=None, len_k=None, prefix
     if slopes is not None and slopes.requires_grad:
         raise ops.E2KError('packed_attention: slopes get no gradient; pass slopes.detach(), or learn a RelativePositionBias')
     table, buckets = (None, None) if bias is None else (bias.weight, bias.buckets)
+    _no_tangents('packed_attention', q, k, v, slopes, table)
     kw = dict(len_q=len_q, len_k=len_k, prefix=prefix, max_q=max_q, max_k=max_k, causal=causal, scale=scale, softcap=softcap, slopes=slopes, buckets=buckets)
     if not torch.is_grad_enabled():              # (nothing is kept for a backward)
         return ops.packed_attn_fwd(q, k, v, cu_q, cu_k, table=table, **kw)
@@ -58,6 +67,7 @@ def packed_attention(q, k, v, cu_q, cu_k=None, *, len_q=None, len_k=None, prefix
 
 def attn_decode(q, k_cache, v_cache, lens, *, scale=None, softcap=0., slopes=None, bias=None, out=None):
     """ops.attn_decode with a RelativePositionBias as its `bias` (no gradients: serving)"""
+    _no_tangents('attn_decode', q, k_cache, v_cache, slopes, None if bias is None else bias.weight)
     table, buckets = (None, None) if bias is None else (bias.weight.detach(), bias.buckets)
     return ops.attn_decode(q.detach(), k_cache.detach(), v_cache.detach(), lens, scale=scale, softcap=softcap, slopes=slopes, table=table, buckets=buckets, out=out)
 
