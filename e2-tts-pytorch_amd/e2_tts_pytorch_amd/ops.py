@@ -1163,8 +1163,13 @@ def rel_buckets(num_buckets=32, max_distance=128, causal=False, device=None):
 
 class PackedAttnState:
     """what packed_attn_fwd(train=True) keeps for packed_attn_bwd"""
-    __slots__ = ('q', 'k', 'v', 'cu_q', 'cu_k', 'len_q', 'len_k', 'prefix', 'max_q', 'max_k', 'causal', 'scale', 'softcap', 'slopes', 'table', 'buckets',
-                 'reach', 'out', 'lo', 'lse2')
+    TENSORS = ('q', 'k', 'v', 'cu_q', 'cu_k', 'len_q', 'len_k', 'prefix', 'slopes', 'table', 'buckets', 'out', 'lo', 'lse2')
+    NUMBERS = ('max_q', 'max_k', 'causal', 'scale', 'softcap', 'reach')
+    __slots__ = TENSORS + NUMBERS
+
+    def __init__(self, **parts):
+        for name in self.__slots__:
+            setattr(self, name, parts[name])
 
 
 def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, len_q=None, len_k=None, prefix=None, max_q=0, max_k=0, causal=False, scale=None, softcap=0., slopes=None,
@@ -1221,10 +1226,8 @@ def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, len_q=None, len_k=None, prefix=
                                        _p(ws), int(fill), _stream(q))
     if not train:
         return out
-    st = PackedAttnState()
-    st.q, st.k, st.v, st.cu_q, st.cu_k, st.len_q, st.len_k, st.prefix, st.max_q, st.max_k = q, k, v, cu_q, cu_k, len_q, len_k, prefix, int(max_q), int(max_k)
-    st.causal, st.scale, st.softcap, st.slopes, st.table, st.buckets, st.reach = bool(causal), scale, softcap, slopes, table, buckets, reach
-    st.out, st.lo, st.lse2 = out, lo, lse2
+    st = PackedAttnState(q=q, k=k, v=v, cu_q=cu_q, cu_k=cu_k, len_q=len_q, len_k=len_k, prefix=prefix, slopes=slopes, table=table, buckets=buckets, out=out, lo=lo,
+                         lse2=lse2, max_q=int(max_q), max_k=int(max_k), causal=bool(causal), scale=scale, softcap=softcap, reach=reach)
     return out, st
 
 

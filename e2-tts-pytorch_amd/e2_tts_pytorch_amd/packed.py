@@ -29,23 +29,17 @@ class _PackedAttnFn(Function):
         if not train:
             return ops.packed_attn_fwd(q, k, v, cu_q, cu_k, table=table, **kw)
         out, st = ops.packed_attn_fwd(q, k, v, cu_q, cu_k, table=table, train=True, **kw)
-        # tensors autograd has to watch (an input or the output changed in place before the backward raises) go through save_for_backward
-        ctx.save_for_backward(q, k, v, table, out, kw['slopes'], kw['buckets'], cu_q, cu_k, kw['len_q'], kw['len_k'], kw['prefix'])
-        st.out = None
-        ctx.st = st
+        # every tensor of the state goes through save_for_backward (changed in place it raises; hooks may pack it away), the numbers beside it
+        ctx.save_for_backward(*(getattr(st, n) for n in st.TENSORS))
+        ctx.numbers = {n: getattr(st, n) for n in st.NUMBERS}
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        saved = ctx.saved_tensors          # (checks the versions)
-        st = ctx.st
-        full = ops.PackedAttnState()
-        for name in ops.PackedAttnState.__slots__:
-            setattr(full, name, getattr(st, name))
-        full.out = saved[4]
+        st = ops.PackedAttnState(**dict(zip(ops.PackedAttnState.TENSORS, ctx.saved_tensors)), **ctx.numbers)
         need = ctx.needs_input_grad
-        dq, dk, dv, dtable = ops.packed_attn_bwd(full, dout, need_table=need[3])
+        dq, dk, dv, dtable = ops.packed_attn_bwd(st, dout, need_table=need[3])
         return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dtable if need[3] else None, None, None, None
 
 

@@ -37,3 +37,49 @@ def test_forward_mode_is_refused(emu, grad):
                 f()
                 print('not refused:', i)
         assert pkg.packed_attention(q, k, v, cu, slopes=slopes).shape == q.shape and pkg.attn_decode(q[:1], kc, kc, n).shape == (1, 2, 64)
+
+
+@pytest.mark.parametrize('table', [False, True], ids=['plain', 'table'])
+def test_saved_tensors_go_through_the_hooks(dev, table, monkeypatch):
+    """all that the backward reads can be packed away: nothing of it stays alive beside the hooks, and what they unpack is what counts"""
+    import gc
+    import weakref
+
+    import e2_tts_pytorch_amd as pkg
+    from e2_tts_pytorch_amd import ops
+    q, k, v, do, cu = attn_inputs(dev)
+    bias = pkg.RelativePositionBias(2, 8, 16).to(dev) if table else None
+    extra = [bias.weight] if table else []
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    want = torch.autograd.grad(pkg.packed_attention(*leaves, cu, bias=bias), leaves + extra, do)
+    kept, plain = [], ops.packed_attn_fwd
+
+    def watched(*a, **kw):
+        out, st = plain(*a, **kw)
+        kept.extend(weakref.ref(t) for t in (st.q, st.k, st.v, st.lo, st.lse2))
+        return out, st
+    monkeypatch.setattr(ops, 'packed_attn_fwd', watched)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: (t.detach().cpu().clone(), t.device), lambda p: p[0].to(p[1])):
+        ins = [t * 1 for t in leaves]
+        ins[1] = torch.cat([ins[1], ins[1]], 2)[..., :64]                    # (read in place, rows 128 apart)
+        ins[2] = ins[2].transpose(1, 2).contiguous().transpose(1, 2)        # (a copy is made)
+        out = pkg.packed_attention(*ins, cu, bias=bias)
+    del ins
+    gc.collect()
+    assert len(kept) == 5 and all(r() is None for r in kept), [i for i, r in enumerate(kept) if r() is not None]
+    with torch.no_grad():
+        out.data.zero_()                                                     # (the packed output is another tensor)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, leaves + extra, do), want))
+
+
+def test_recomputed_in_the_backward(dev):
+    """under non-reentrant checkpointing: the same gradients"""
+    from torch.utils.checkpoint import checkpoint
+
+    import e2_tts_pytorch_amd as pkg
+    q, k, v, do, cu = attn_inputs(dev)
+    bias = pkg.RelativePositionBias(2, 8, 16).to(dev)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)] + [bias.weight]
+    f = lambda q, k, v: pkg.packed_attention(q, k, v, cu, bias=bias, causal=True)  # noqa: E731
+    want = torch.autograd.grad(f(*leaves[:3]), leaves, do)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(checkpoint(f, *leaves[:3], use_reentrant=False), leaves, do), want))
