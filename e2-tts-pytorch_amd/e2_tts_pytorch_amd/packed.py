@@ -86,11 +86,17 @@ class RelativePositionBias(nn.Module):
         return self.weight[self.buckets.long()[d.clamp(-self.reach, self.reach) + self.reach]].permute(2, 0, 1)
 
 
+def _ln_input(x):
+    """x as rows that the kernels can read in place, a copy where its last dimension is strided or its rows overlap"""
+    rows = x.reshape(-1, x.shape[-1])
+    M, D = rows.shape
+    return rows.contiguous() if (D > 1 and rows.stride(1) != 1) or (M > 1 and rows.stride(0) < D) else rows
+
+
 class _LayerNormFn(Function):
     @staticmethod
     def forward(ctx, x, gamma, beta, gamma_off, rows_per_batch, eps):
-        rows = x.reshape(-1, x.shape[-1])
-        y, mean, rstd = ops.layernorm_fwd(rows, gamma, beta, gamma_off, rows_per_batch, eps)
+        y, mean, rstd = ops.layernorm_fwd(_ln_input(x), gamma, beta, gamma_off, rows_per_batch, eps)
         ctx.save_for_backward(x, gamma, mean, rstd)
         ctx.args = gamma_off, rows_per_batch, None if gamma is None else gamma.shape, None if beta is None else beta.shape
         return y.view(x.shape)
@@ -102,7 +108,7 @@ class _LayerNormFn(Function):
         off, rpb, gs, bs = ctx.args
         need = ctx.needs_input_grad
         D = x.shape[-1]
-        dx, dg, db = ops.layernorm_bwd(dy.reshape(-1, D).to(x.dtype), x.reshape(-1, D), mean, rstd, gamma, off, rpb, need_weights=need[1] or need[2])
+        dx, dg, db = ops.layernorm_bwd(dy.reshape(-1, D).to(x.dtype), _ln_input(x), mean, rstd, gamma, off, rpb, need_weights=need[1] or need[2])
 
         def shaped(t, shape):            # rows of gamma / beta beyond the last batch element are not read: zero gradient
             if t.shape[0] == (1 if len(shape) == 1 else shape[0]):

@@ -83,3 +83,25 @@ def test_recomputed_in_the_backward(dev):
     f = lambda q, k, v: pkg.packed_attention(q, k, v, cu, bias=bias, causal=True)  # noqa: E731
     want = torch.autograd.grad(f(*leaves[:3]), leaves, do)
     assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(checkpoint(f, *leaves[:3], use_reentrant=False), leaves, do), want))
+
+
+def test_layer_norm_of_views(dev):
+    """transposed, expanded and column-strided inputs of two and three dimensions, an input gradient that is one of them: as the contiguous copy"""
+    import e2_tts_pytorch_amd as pkg
+    g = torch.Generator().manual_seed(1)
+    gam, bet = (torch.randn(8, generator=g).to(dev) for _ in range(2))
+    base = torch.randn(8, 6, 8, generator=g).to(dev)
+    for make in (lambda b: b[0, :6, :6].t().contiguous().t()[:, :6], lambda b: b[:, 0].t(), lambda b: b[0, :1].expand(5, 8), lambda b: b[:, :, ::2], lambda b: b[0, :, ::2],
+                 lambda b: b.transpose(0, 2), lambda b: b[0, 0], lambda b: b[0, 0].expand(2, 3, 8), lambda b: b[0, 0, :1].expand(8), lambda b: b[:0, 0].expand(0, 8)):
+        for dt in (f32, bf16):
+            x = make(base.to(dt))
+            D = x.shape[-1]
+            dy = make(torch.randn(8, 6, 8, generator=torch.Generator().manual_seed(2)).to(dev).to(dt))
+            outs = []
+            for xi, dyi in ((x, dy), (x.contiguous(), dy.contiguous())):
+                xi = xi.detach().requires_grad_()
+                w, b = gam[:D].clone().requires_grad_(), bet[:D].clone().requires_grad_()
+                y = pkg.layer_norm(xi, w, b)
+                outs.append([y, *torch.autograd.grad(y, [xi, w, b], dyi)])
+            assert outs[0][0].shape == x.shape and outs[0][1].shape == x.shape
+            assert all(torch.equal(s, t) for s, t in zip(*outs)), (tuple(x.shape), x.stride(), dt)
