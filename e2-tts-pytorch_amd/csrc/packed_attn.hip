@@ -990,7 +990,7 @@ int check(const PAArgs& a) {
     if (!(a.scale > 0.f) || !(a.cap >= 0.f) || !(a.scale < 1e30f) || !(a.cap < 1e30f)) return E2K_ERR_ARG;
     if (a.slopes && a.table) return E2K_ERR_ARG;
     if (a.table && (!a.buckets || a.nbuckets < 1 || a.R < 0 || a.R > REACH_MAX)) return E2K_ERR_SHAPE;
-    if (!a.Q || (a.Tk > 0 && (!a.K || !a.V))) return E2K_ERR_ARG;
+    if ((a.Tq > 0 && !a.Q) || (a.Tk > 0 && (!a.K || !a.V))) return E2K_ERR_ARG;
     if (!strides_ok(a.sq, a.hq) || !strides_ok(a.sk, a.hk) || !strides_ok(a.sv, a.hv) || !strides_ok(a.so, a.ho)) return E2K_ERR_ALIGN;
     if (!aligned16(a.Q) || !aligned16(a.K) || !aligned16(a.V) || !aligned16(a.O)) return E2K_ERR_ALIGN;
     return E2K_OK;
@@ -1098,9 +1098,9 @@ int packed_attn_bwd_impl(const void* dO, int64_t sg, int64_t hg, const void* Q, 
     a.dQ = (bf16_t*)dQ; a.dK = (bf16_t*)dK; a.dV = (bf16_t*)dV; a.dist = ws; a.fill = fill_gaps;
     hipStream_t st = (hipStream_t)stream;
     long grid;
+    const int rc = check(a);                   // (also without queries: keys are read and their gradients written all the same)
+    if (rc) return rc;
     if (Tq > 0) {
-        const int rc = check(a);
-        if (rc) return rc;
         if (!dO || !O || !Olo || !lse2 || !delta || !dQ || (dtable && (!table || !ws))) return E2K_ERR_ARG;
         if (!strides_ok(sg, hg) || !aligned16(dO) || !aligned16(Olo) || !aligned16(dQ) || !aligned16(dK) || !aligned16(dV)) return E2K_ERR_ALIGN;
         if (Tk > 0 && (!dK || !dV)) return E2K_ERR_ARG;
@@ -1111,8 +1111,6 @@ int packed_attn_bwd_impl(const void* dO, int64_t sg, int64_t hg, const void* Q, 
             PA_PICK(run_dq, a, dtable ? (reach <= 128 ? 1 : 2) : 0, grid, st);
             E2K_CHECK_LAUNCH();
         }
-    } else if (nd < 0 || Tk < 0 || H < 1 || Hkv < 1 || H % Hkv != 0) {
-        return E2K_ERR_SHAPE;
     }
     float* rest = ws;                          // workspace behind the table's part
     if (dtable) {

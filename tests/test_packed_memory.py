@@ -107,3 +107,26 @@ def test_contiguous_but_misaligned_tensors_are_copied(dev):
     cu = offsets([1], dev)
     assert torch.equal(ops.packed_attn_fwd(one, one, one, cu), ops.packed_attn_fwd(q[:1], q[:1], q[:1], cu))
     assert torch.equal(ops.attn_decode(one, k[:1], v[:1], n[:1]), ops.attn_decode(q[:1], k[:1], v[:1], n[:1]))
+
+
+def test_backward_without_queries_checks_its_keys(emu):
+    """the C entry with no query rows still writes dk and dv: pointers, strides and sizes are held to the same rules (the missing ones after the others: each
+    is refused before a kernel could follow it)"""
+    from e2_tts_pytorch_amd import _lib, ops
+    k = torch.zeros(6, 2, 64, dtype=bf16)
+    dk, dv, cu = torch.ones_like(k), torch.ones_like(k), torch.zeros(2, dtype=torch.int32)
+    cuk = torch.tensor([0, 6], dtype=torch.int32)
+    names = 'dO sg hg Q sq hq K sk hk V sv hv cu_q cu_k len_q len_k prefix nd Tq Tk H Hkv max_q max_k causal scale softcap slopes table buckets nbuckets reach O so ho Olo lse2 delta dQ dK dV dtable accumulate ws fill stream'.split()
+    good = dict.fromkeys(names, 0) | dict.fromkeys('dO Q len_q len_k prefix slopes table buckets O Olo lse2 delta dQ dtable ws stream'.split(), None)
+    good |= dict(sg=128, hg=64, sq=128, hq=64, K=k.data_ptr(), sk=128, hk=64, V=k.data_ptr(), sv=128, hv=64, cu_q=cu.data_ptr(), cu_k=cuk.data_ptr(), nd=1, Tk=6, H=2,
+                 Hkv=2, scale=0.125, softcap=0., so=128, ho=64, dK=dk.data_ptr(), dV=dv.data_ptr(), fill=1)
+
+    def call(**other):
+        _lib.get().e2k_packed_attn_bwd(*(good | other).values())
+    call()
+    assert (dk == 0).all() and (dv == 0).all()
+    for other in (dict(sk=127), dict(hv=60), dict(K=k.data_ptr() + 2), dict(scale=0.), dict(softcap=-1.), dict(H=3, Hkv=2), dict(nd=-1), dict(cu_q=None), dict(cu_k=None), dict(K=None),
+                  dict(V=None), dict(dK=None)):
+        with pytest.raises(ops.E2KError):
+            call(**other)
+            print('not refused:', other)
