@@ -57,7 +57,7 @@ struct PAArgs {
     bf16_t* O; void* Olo;                              // O strided; Olo (Tq, H, 64): fp32 with a table, else bf16
     float *lse2, *delta;                               // (H, Tq)
     bf16_t *dQ, *dK, *dV;                              // (Tq, H, 64), (Tk, Hkv, 64)
-    float* dist;                                       // [workgroup of the dQ grid][2 R + 1]: sums of dS by distance
+    float* dist;                                       // [head][row of a (document, tile): dist_row][2 R + 1]: sums of dS by distance
     int nt, nwork, heads, order;                       // row tiles per (document, head) of this grid; workgroups that compute; heads x parts; longest
                                                        // documents first
     int splits; float* part;                           // parts of a tile's sweep; dK / dV: their sums [part][dK | dV][Tk][Hkv][64]; forward: their
@@ -107,7 +107,7 @@ __device__ __forceinline__ int doc_of_rank(const int* cu, const int* len, int nd
 // more workgroups than slots the long sweeps go first (cu / len: the axis that a workgroup sweeps, whose length is the workgroup's time) and a
 // document's heads side by side: 11 documents of 97 .. 1056 tokens in a mixed order, forward 91 -> 88 us, dQ 118 -> 116, dK / dV 123 -> 119; six of
 // 1056 and 2112, causal, forward 89 -> 80, dQ 101 -> 96.  A dK / dV sweep in parts is better off as the documents lie (131 against 141 us there).
-struct Work { int h, d, tile, lin; };
+struct Work { int h, d, tile; };
 __device__ __forceinline__ Work work_of(const PAArgs& p, const int* cu, const int* len, int total) {
     const int q = p.nwork >> 3, r = p.nwork & 7;
     const int xcd = (int)blockIdx.x & 7, in = (int)blockIdx.x >> 3;
@@ -125,7 +125,6 @@ __device__ __forceinline__ Work work_of(const PAArgs& p, const int* cu, const in
     }
     w.tile = p.nt - 1 - w.tile;              // causal: the long rows first
     if (p.order) w.d = doc_of_rank(cu, len, p.nd, total, w.d);
-    w.lin = (w.h * p.nd + w.d) * p.nt + p.nt - 1 - w.tile;
     return w;
 }
 
@@ -514,6 +513,12 @@ __device__ __forceinline__ void diag_add(const float (&ds)[16], float* scr, floa
     dist_at_lo[hi ? l31 - 32 : l31] += hi ? B : A;
 }
 
+// Sums by distance of one head: a row of 2 R + 1 for each tile of each document with rows, however large the grid is (most of its workgroups are empty where
+// the longest document is not known).  A document of n rows from row `at` on has tiles at / 128 + min(d, at) .. + ceil(n / 128) - 1: the next one with rows starts
+// at least n >= 1 rows further on, so that floor((at + n) / 128) - floor(at / 128) + 1 >= ceil(n / 128) tiles lie between them.
+__host__ __device__ __forceinline__ long dist_rows(int nd, int Tq) { return Tq / 128 + (nd < Tq ? nd : Tq); }
+__device__ __forceinline__ int dist_row(int d, int at) { return at / 128 + min(d, at); }
+
 constexpr int distn(int reach) { return 2 * reach + 1 + 2 * PADL; }
 
 // Lane layout and ring of the forward; dP beside the scores, dQ^T = K^T dS^T from the same K tile.  8 x 1056 tokens x 16 heads, no bias: 74 us; with a
@@ -697,7 +702,7 @@ __global__ __launch_bounds__(256, (BIAS || CAP) ? 2 : 3) void pa_dq_kernel(PAArg
             mydist[PADL + 2 * p.R] += far_hi + b;
         }
         __syncthreads();
-        float* out = p.dist + (long)wk.lin * (2 * p.R + 1);
+        float* out = p.dist + (h * dist_rows(p.nd, p.Tq) + dist_row(wk.d, D.q0) + wk.tile) * (2 * p.R + 1);
         for (int i = tid; i < 2 * p.R + 1; i += 256) {
             const float* d = dist + PADL + i;
             out[i] = (d[0] + d[ND]) + (d[2 * ND] + d[3 * ND]);
@@ -705,17 +710,47 @@ __global__ __launch_bounds__(256, (BIAS || CAP) ? 2 : 3) void pa_dq_kernel(PAArg
     }
 }
 
-// sums over the workgroups of a head -> by_dist[h][2 R + 1]; 64 distances x 16 row groups per workgroup (6 us: latency of its dependent loads)
+// sums over the tiles of a head -> by_dist[h][2 R + 1]; 64 distances x 16 row groups per workgroup (6 us: latency of its dependent loads).  64 documents at a
+// time: their rows are listed (a thread each finds its document by bisection), then added in the list's order
 __global__ __launch_bounds__(1024) void pa_dist_reduce_kernel(PAArgs p, float* by_dist) {
     __shared__ float sm[16][64];
-    const int lane = threadIdx.x & 63, grp = threadIdx.x >> 6, h = blockIdx.y;
+    __shared__ int first[64], tiles[64], upto[65], list[1024];
+    const int tid = threadIdx.x, lane = tid & 63, grp = tid >> 6, h = blockIdx.y;
     const int N = 2 * p.R + 1, i = blockIdx.x * 64 + lane;
     float a = 0.f;
-    const float* q = p.dist + (long)h * p.nd * p.nt * N + i;
+    const float* q = p.dist + h * dist_rows(p.nd, p.Tq) * N + i;
+    for (int d0 = 0; d0 < p.nd; d0 += 64) {
+        const int nd = min(64, p.nd - d0);
+        if (tid < nd) {
+            const Span s = span(p.cu_q, p.len_q, d0 + tid, p.Tq);
+            first[tid] = dist_row(d0 + tid, s.at);
+            tiles[tid] = min((s.n + 127) / 128, p.nt);            // (a workgroup takes the tiles from nt on into its first one's row)
+        }
+        __syncthreads();
+        if (tid <= nd) {
+            int sum = 0;
+            for (int j = 0; j < tid; ++j) sum += tiles[j];
+            upto[tid] = sum;
+        }
+        __syncthreads();
+        const int total = upto[nd];
+        for (int seg = 0; seg < total; seg += 1024) {
+            const int f = seg + tid, n = min(1024, total - seg);
+            if (f < total) {
+                int j = 0, end = nd;                               // upto[j] <= f < upto[end]
+                while (end - j > 1) {
+                    const int mid = (j + end) / 2;
+                    if (upto[mid] <= f) j = mid; else end = mid;
+                }
+                list[tid] = first[j] + f - upto[j];
+            }
+            __syncthreads();
+            if (i < N) {
 #pragma unroll 4
-    for (int w = grp; w < p.nd * p.nt; w += 16) {
-        const int t = p.nt - 1 - w % p.nt;                        // (Work::tile of this row of partial sums)
-        if (i < N && t * 128 < span(p.cu_q, p.len_q, w / p.nt, p.Tq).n) a += q[(long)w * N];
+                for (int w = grp; w < n; w += 16) a += q[(long)list[w] * N];
+            }
+            __syncthreads();
+        }
     }
     sm[grp][lane] = a;
     __syncthreads();
@@ -1116,15 +1151,13 @@ int packed_attn_bwd_impl(const void* dO, int64_t sg, int64_t hg, const void* Q, 
     if (dtable) {
         if (!table || !buckets || !ws || nbuckets < 1 || reach < 0 || reach > REACH_MAX) return E2K_ERR_ARG;
         const int N = 2 * reach + 1;
-        const long nq_work = a.nwork;
-        float* by_dist = ws + (Tq > 0 ? nq_work * N : 0);
-        if (Tq == 0) a.nd = 0;                 // nothing was written: the sums are empty
+        const long sums = H * dist_rows(nd, Tq) * N;          // (no query rows: none, and no tiles to add)
+        float* by_dist = ws + sums;
         hipLaunchKernelGGL(pa_dist_reduce_kernel, dim3((N + 63) / 64, H), dim3(1024), 0, st, a, by_dist);
         E2K_CHECK_LAUNCH();
         hipLaunchKernelGGL(pa_table_grad_kernel, dim3((nbuckets * H + 3) / 4), dim3(256), 0, st, by_dist, buckets, N, nbuckets, H, dtable, accumulate);
         E2K_CHECK_LAUNCH();
-        a.nd = nd;
-        rest = ws + (((Tq > 0 ? (long)nq_work * N : 0) + (long)H * N + 3) / 4 * 4);          // (16-byte rows)
+        rest = ws + (sums + (long)H * N + 3) / 4 * 4;          // (16-byte rows)
     }
     if (Tk > 0) {
         if (!dK || !dV || !aligned16(dK) || !aligned16(dV)) return E2K_ERR_ARG;
@@ -1169,8 +1202,7 @@ int64_t e2k_query_packed_attn_bwd_ws_floats(int nd, int Tq, int Tk, int H, int H
     const int s = splits_for(Tk, H, Hkv, max_q, Tq);
     const int64_t join = s > 1 ? (int64_t)s * 2 * Tk * Hkv * DH : 0;
     if (!dtable) return join;
-    const int64_t wgs = Tq > 0 ? (int64_t)nd * tiles_for(max_q, Tq, nd, H) * H : 0;
-    const int64_t sums = (wgs + H) * (2 * (int64_t)reach + 1);
+    const int64_t sums = H * (dist_rows(nd, Tq) + 1) * (2 * (int64_t)reach + 1);
     return (sums + 3) / 4 * 4 + join;
 }
 int e2k_packed_attn_bwd(const void* dO, int64_t sg, int64_t hg, const void* Q, int64_t sq, int64_t hq, const void* K, int64_t sk, int64_t hk,

@@ -130,3 +130,27 @@ def test_backward_without_queries_checks_its_keys(emu):
         with pytest.raises(ops.E2KError):
             call(**other)
             print('not refused:', other)
+
+
+def test_workspace_of_the_table_gradient(emu):
+    """sized by the rows and documents there are: a hint that is missing costs nothing"""
+    from e2_tts_pytorch_amd import _lib
+    f = _lib.get().e2k_query_packed_attn_bwd_ws_floats
+    for max_q in (0, 1024, 16384):
+        for nd, T, H, reach in ((64, 16384, 16, 512), (128, 16384, 16, 512), (1, 16384, 16, 128), (70000, 340, 2, 128)):
+            join = f(nd, T, T, H, H, max_q, 0, 0)
+            assert f(nd, T, T, H, H, max_q, reach, 1) - join <= H * (T // 128 + min(nd, T) + 1) * (2 * reach + 1) + 3
+
+
+@pytest.mark.parametrize('hint', [0, 130, 1])
+def test_table_gradient_over_tiles_and_documents(dev, hint):
+    """documents that start anywhere in a tile, empty ones, more than 64 of them, slots longer than their documents: the same sums whatever the hint (to
+    their order), and the same bits twice"""
+    for kw in (dict(ql=[130, 0, 126, 1, 0, 255, 128, 3]), dict(ql=[1, 0, 2] * 43 + [200]), dict(ql=[140, 300, 20], kl=[150, 290, 20], nq=[129, 130, 0], nk=[150, 3, 20])):
+        c = Case(H=1, bias='table', buckets=6, reach=10, **kw)
+        from test_packed_attn import run
+        got = run(c, dev, max_q=hint)
+        want, bound = c.exact()
+        for n in want:
+            held(got[n], want[n], bound[n], n)
+        assert torch.equal(got['dtable'], run(c, dev, max_q=hint)['dtable'])
