@@ -764,6 +764,8 @@ def layernorm_bwd(dy, x, mean, rstd, gamma, gamma_off=0., rows_per_batch=0, dgam
             _ln_cols(dgamma, x, rpb, 'dgamma', True), _ln_cols(dbeta, x, rpb, 'dbeta', True)
             if dgamma.shape != dbeta.shape or dgamma.stride() != dbeta.stride():
                 raise E2KError('layer norm: dgamma and dbeta must have the same shape and strides')
+            if _rows_meet(dgamma, dbeta):
+                raise E2KError('layer norm: dgamma and dbeta share memory')
         ldd = dgamma.stride(0) if dgamma.dim() == 2 else D
         ws = torch.empty(_lib.get().e2k_query_layernorm_bwd_ws_floats(M, D, rpb), dtype=f32, device=x.device)
     elif dgamma is not None or dbeta is not None:
@@ -1252,6 +1254,8 @@ def packed_attn_bwd(st, dout, dtable=None, need_table=True):
             dtable = torch.empty_like(st.table)
         elif dtable.dtype != f32 or dtable.shape != st.table.shape or not dtable.is_contiguous() or dtable.device != dev:
             raise E2KError('packed attention: dtable must be contiguous fp32 like the table')
+        elif _rows_meet(dtable, st.table):
+            raise E2KError('packed attention: dtable shares memory with the table')
         else:
             acc = 1
     n = _lib.get().e2k_query_packed_attn_bwd_ws_floats(nd, Tq, Tk, H, Hkv, st.max_q, st.reach, int(dtable is not None))

@@ -154,3 +154,22 @@ def test_table_gradient_over_tiles_and_documents(dev, hint):
         for n in want:
             held(got[n], want[n], bound[n], n)
         assert torch.equal(got['dtable'], run(c, dev, max_q=hint)['dtable'])
+
+
+def test_gradient_buffers_that_share_memory_are_refused(emu):
+    """a table's gradient added into the table (still read by the kernel that follows), a scale's and a shift's into one buffer"""
+    from e2_tts_pytorch_amd import ops
+    c = Case([10], bias='table')
+    a, kw = c.args('cpu')
+    out, st = ops.packed_attn_fwd(*a, train=True, **kw)
+    with pytest.raises(ops.E2KError):
+        ops.packed_attn_bwd(st, c.dout, dtable=kw['table'])
+    x, w = torch.randn(6, 8), torch.ones(3, 8)
+    y, m, r = ops.layernorm_fwd(x, w, w, 0., 2)
+    both = torch.zeros(4, 2, 8)
+    for dg, db in ((both[:3, 0], both[:3, 0]), (both[:3, 0], both[1:, 0]), (both.view(8, 8)[:3], both.view(8, 8)[2:5])):
+        with pytest.raises(ops.E2KError):
+            ops.layernorm_bwd(x, x, m, r, w, 0., 2, dg, db)
+    want = ops.layernorm_bwd(x, x, m, r, w, 0., 2)
+    got = ops.layernorm_bwd(x, x, m, r, w, 0., 2, both[:3, 0], both[:3, 1])
+    assert all(torch.equal(s, t) for s, t in zip(got, want)) and (both[3] == 0).all()
