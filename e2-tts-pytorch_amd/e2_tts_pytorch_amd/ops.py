@@ -1110,9 +1110,18 @@ def _heads64(t, what):
 def _apart(out, q, k, v, what, in_place):
     """refuses an output that shares memory with what other workgroups still read.  in_place: it may be q itself (a row of q is read by the workgroups
     that its output row waits for, and by no other)"""
-    same = in_place and out.data_ptr() == q.data_ptr() and all(n == 1 or s == t for n, s, t in zip(q.shape, q.stride(), out.stride()))
-    if (not same and _rows_meet(out, q)) or _rows_meet(out, k) or _rows_meet(out, v):
-        raise E2KError(f'{what}: out shares memory with ' + ('k or v, or with q without being it' if in_place else 'q, k or v'))
+    mem = out.untyped_storage()
+    lo = mem.data_ptr()
+    hi = lo + mem.nbytes()
+    for t in (q, k, v):
+        mem = t.untyped_storage()
+        at = mem.data_ptr()
+        if at >= hi or at + mem.nbytes() <= lo:               # (allocations of their own: the usual case, 3 us for all of it)
+            continue
+        if t is q and in_place and out.data_ptr() == q.data_ptr() and all(n == 1 or x == y for n, x, y in zip(q.shape, q.stride(), out.stride())):
+            continue
+        if _rows_meet(out, t):
+            raise E2KError(f'{what}: out shares memory with ' + ('k or v, or with q without being it' if in_place else 'q, k or v'))
 
 
 def _offsets(cu, what, device, n=None):
@@ -1211,7 +1220,7 @@ def packed_attn_fwd(q, k, v, cu_q, cu_k=None, *, len_q=None, len_k=None, prefix=
         out = torch.empty((Tq, H, 64), dtype=bf16, device=dev)
     else:
         if out.shape != q.shape or out.dtype != bf16 or out.device != dev or out.stride(2) != 1 or out.stride(0) % 8 or out.stride(1) % 8 or out.data_ptr() % 16 \
-                or out.stride(0) >= 1 << 23 or _row_dims(out) is None:
+                or out.stride(0) >= 1 << 23 or not (out.is_contiguous() or _row_dims(out) is not None):
             raise E2KError('packed attention: out must be a (Tq, H, 64) bf16 tensor like q with 16-byte rows that do not overlap')
         _apart(out, q, k, v, 'packed attention', not train)
     lo = lse2 = ws = None
@@ -1298,7 +1307,7 @@ def attn_decode(q, k_cache, v_cache, lens, *, scale=None, softcap=0., slopes=Non
     if out is None:
         out = torch.empty((B, H, 64), dtype=bf16, device=dev)
     else:
-        if out.shape != (B, H, 64) or out.dtype != bf16 or out.stride(2) != 1 or out.device != dev or _row_dims(out) is None:
+        if out.shape != (B, H, 64) or out.dtype != bf16 or out.stride(2) != 1 or out.device != dev or not (out.is_contiguous() or _row_dims(out) is not None):
             raise E2KError('attn_decode: out must be (sequences, heads, 64) bf16 like q, with contiguous rows that do not overlap')
         _apart(out, q, k_cache, v_cache, 'attn_decode', True)
     L = _lib.get()
