@@ -274,7 +274,7 @@ int attn_decode_impl(const void* Q, int64_t qb, int64_t qh, const void* K, int64
     if (B < 0 || capacity < 0 || H < 1 || Hkv < 1 || H % Hkv != 0) return E2K_ERR_SHAPE;
     if (B == 0) return E2K_OK;
     if (!Q || !O || !lens || (capacity > 0 && (!K || !V))) return E2K_ERR_ARG;
-    if (!(scale > 0.f) || !(scale < 1e30f) || !(softcap >= 0.f) || !(softcap < 1e30f) || (slopes && table)) return E2K_ERR_ARG;
+    if (!score_range_ok(scale, softcap) || (slopes && table)) return E2K_ERR_ARG;
     if (table && (!buckets || nbuckets < 1 || reach < 0)) return E2K_ERR_SHAPE;
     if (!aligned16(Q) || !aligned16(K) || !aligned16(V) || !ok8(qb) || !ok8(qh) || !ok8(kb) || !ok8(kn) || !ok8(kh) || !ok8(vb) || !ok8(vn) || !ok8(vh))
         return E2K_ERR_ALIGN;

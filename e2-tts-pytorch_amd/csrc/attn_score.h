@@ -21,6 +21,8 @@ __device__ __forceinline__ constexpr int reg_off(int r) { return 16 * (r >> 3) +
 // a score is below 3e-5 at any cap up to 50); beyond: 1 - 2 / (2^(2 x log2 e) + 1), absolute error 2^-22
 constexpr float CAP_POLY_MAX = 0.3f;
 struct Cap { float a0, a1, a2, a3, k2, out, lim; };
+// what the kernels' fp32 arithmetic takes: scale / cap and its products with scores stay finite or saturate
+inline bool score_range_ok(float scale, float cap) { return scale > 0.f && scale < 1e30f && (cap == 0.f || (cap >= 1e-30f && cap < 1e30f && scale / cap < 1e30f)); }
 template <bool FINE> __device__ __forceinline__ Cap cap_of(float scale, float cap) {
     Cap c;
     const float kx = scale / cap, k2 = kx * kx;
@@ -31,7 +33,7 @@ template <bool FINE> __device__ __forceinline__ Cap cap_of(float scale, float ca
     c.a2 = k1 * k2 * k2 * (FINE ? 0.13312598f : 0.12633947f);
     c.a3 = FINE ? k1 * k2 * k2 * k2 * -0.050222438f : 0.f;
     c.k2 = 2.f * LOG2E * kx;
-    c.lim = CAP_POLY_MAX / kx;
+    c.lim = k1 * k2 * k2 * k2 < 1e37f ? CAP_POLY_MAX / kx : -1.f;      // (a cap of next to nothing: coefficients that overflow make 0 times infinity of a score of 0)
     return c;
 }
 // x[r] = capped z[r] + add(r), and with KEEP z[r] capped in place (the backward's 1 - tanh^2)

@@ -1022,7 +1022,7 @@ bool strides_ok(long t, long h) { return t % 8 == 0 && h % 8 == 0 && t >= 0 && h
 int check(const PAArgs& a) {
     if (a.nd < 0 || a.Tq < 0 || a.Tk < 0 || a.H < 1 || a.Hkv < 1 || a.H % a.Hkv != 0) return E2K_ERR_SHAPE;
     if (a.nd > 0 && (!a.cu_q || !a.cu_k)) return E2K_ERR_ARG;
-    if (!(a.scale > 0.f) || !(a.cap >= 0.f) || !(a.scale < 1e30f) || !(a.cap < 1e30f)) return E2K_ERR_ARG;
+    if (!score_range_ok(a.scale, a.cap)) return E2K_ERR_ARG;
     if (a.slopes && a.table) return E2K_ERR_ARG;
     if (a.table && (!a.buckets || a.nbuckets < 1 || a.R < 0 || a.R > REACH_MAX)) return E2K_ERR_SHAPE;
     if ((a.Tq > 0 && !a.Q) || (a.Tk > 0 && (!a.K || !a.V))) return E2K_ERR_ARG;

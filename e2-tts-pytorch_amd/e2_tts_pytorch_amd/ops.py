@@ -1134,8 +1134,8 @@ def _score_args(H, device, scale, softcap, slopes, table, buckets, what='packed 
     """checks of the score's options -> (scale, softcap, number of buckets, reach)"""
     scale = 0.125 if scale is None else float(scale)
     softcap = float(softcap)
-    if not 0. < scale < 1e30 or not 0. <= softcap < 1e30:
-        raise E2KError(f'{what}: scale must be positive and softcap not negative, got {scale}, {softcap}')
+    if not 0. < scale < 1e30 or not (softcap == 0. or (1e-30 <= softcap < 1e30 and scale / softcap < 1e30)):
+        raise E2KError(f'{what}: scale must be positive, softcap 0 or positive (1e-30 at least, and scale / softcap below 1e30), got {scale}, {softcap}')
     if slopes is not None and table is not None:
         raise E2KError(f'{what}: slopes or a table, not both')
     if slopes is not None and (slopes.dtype != f32 or slopes.shape != (H,) or not slopes.is_contiguous() or slopes.device != device):

@@ -352,7 +352,7 @@ int e2k_freq_attn_bwd(const void* dout, const void* qkv, int64_t ld, const void*
  * device, never falling; offsets outside the tensors are cut off); len_q / len_k (device, may be NULL): only the first len rows of each slot
  * count.  Query i of nq stands at position i + nk - nq.  It sees every key of its document (causal = 0), or the keys up to its position and the
  * first prefix[d] keys (causal = 1; prefix device, may be NULL).
- *   z = scale q.k;  c = softcap tanh(z / softcap) (softcap > 0, else z);  t = c - slopes[h] |j - i|  or  t = c + table[buckets[clamp(j - i) + reach]][h]
+ *   z = scale q.k;  c = softcap tanh(z / softcap) (softcap > 0: 1e-30 at least, scale / softcap < 1e30; else z);  t = c - slopes[h] |j - i|  or  t = c + table[buckets[clamp(j - i) + reach]][h]
  * (positions; slopes fp32 (H); table fp32 (nbuckets, H); buckets int32 (2 reach + 1) by key minus query distance, clamped at +-reach <= 512; one of
  * slopes / table or neither), softmax over the visible keys, O = P V; a row that sees nothing is 0.  A bias of -1e30 or less hides its keys.
  * O (Tq, H, 64) strided; rows that no document covers are zeroed with fill_gaps = 1, left alone with 0.  For the backward: Olo

@@ -98,3 +98,34 @@ def test_training_forward_of_one_dominating_key(dev, bias, cap):
 
 def test_training_forward_grouped_heads(dev):
     check(Case([90], H=4, Hkv=2, mask='causal', bias='alibi', gain=8.), dev)
+
+
+@pytest.mark.parametrize('bias', BIASES)
+@pytest.mark.parametrize('cap', [1e-3, 1e-9, 1e-20, 1e-28, 1e29])
+def test_caps_far_from_the_scores(dev, bias, cap):
+    """a cap of next to nothing leaves the bias alone, one far above every score changes nothing; whole blocks of scores that are exactly zero among them"""
+    from e2_tts_pytorch_amd import ops
+    c = Case([70, 9], cap=cap, bias=bias)
+    c.q[:64] = 0
+    want, _ = c.exact()
+    a, kw = c.args(dev)
+    out, st = ops.packed_attn_fwd(*a, train=True, **kw)
+    got = dict(zip(('dq', 'dk', 'dv'), ops.packed_attn_bwd(st, c.dout.to(dev)))) | dict(out=out, inference=ops.packed_attn_fwd(*a, **kw))
+    kc, vc = a[1][None, :70], a[2][None, :70]
+    got['decode'] = ops.attn_decode(a[0][:1], kc, vc, torch.tensor([1], dtype=torch.int32, device=dev), softcap=cap, slopes=kw['slopes'], table=kw['table'], buckets=kw['buckets'])
+    want['inference'], want['decode'] = want['out'], a[2][:1].cpu().to(f64)
+    for n, t in got.items():
+        # P, dS, dO.o and the result are each rounded to bf16: four half steps of sums of magnitudes below 4 |v| |k| sqrt(79)
+        held(t, want[n], 4 * HALF * (want[n].abs() + 1), n)
+
+
+def test_caps_out_of_range_are_refused(emu):
+    from e2_tts_pytorch_amd import ops
+    c = Case([8])
+    a, _ = c.args('cpu')
+    n = torch.tensor([8], dtype=torch.int32)
+    for scale, cap in ((0.125, 1e-38), (1e20, 1e-12), (0.125, 1e-42)):
+        with pytest.raises(ops.E2KError):
+            ops.packed_attn_fwd(*a, scale=scale, softcap=cap)
+        with pytest.raises(ops.E2KError):
+            ops.attn_decode(a[0][:1], a[1][None], a[2][None], n, scale=scale, softcap=cap)
