@@ -24,8 +24,9 @@
 // The backward works with small differences p (dO.v - dO.o), and the table's gradient is a sum of them over every pair at a distance, in fp32: an
 // o that is good to bf16 only (probabilities rounded before the second product, output rounded after it) shows in the gradients of q and k (2.9e-3
 // off the exact ones instead of 2.4e-3) and in the third digit of the table's.  A training forward therefore carries the probabilities as two bf16
-// terms through the second product and keeps what rounding cut off the output (o_lo, bf16); with a table as three terms and o_lo in fp32 (its
-// gradient is then 6e-7 off, as in plain fp32, instead of 3e-6; 89 -> 101 us on 8397 tokens of 11 documents, 16 heads).
+// terms through the second product, sums them unrounded and keeps what rounding cut off the output (o_lo, bf16; out + o_lo is 3e-6 off, on peaked rows
+// too); with a table as three terms and o_lo in fp32 (its gradient is then 8e-7 off, as in plain fp32, instead of 3e-6; 89 -> 101 us on 8397 tokens of
+// 11 documents, 16 heads).
 //
 // Sums are taken in a fixed order throughout: no atomics, the same bits every time.
 #include "e2k_device.h"
@@ -232,8 +233,8 @@ struct Stager {
 // cuts a row's keys into parts and joins them.
 // One workgroup = 128 queries of one (document, head): 4 waves x 32; K / V tiles of 64 keys through a three-stage LDS-DMA ring (two tiles in flight
 // while one is computed: with one, the copies' latency of about 1 us set the pace; one raw barrier a tile), three workgroups a CU.
-// Bound by the vector ALU (88 % of its busy clocks on long rows): 16417 tokens x 16 heads, linear bias, cap: 1.96 ms, 562 TFLOP/s; 8 x 1056 tokens x
-// 16 heads, no bias: 59 us, 618 TFLOP/s (83 with the training form's second term).
+// Bound by the vector ALU (85 % of the clocks in which a CU has work, on long rows): 16417 tokens x 16 heads, linear bias, cap: 1.95 .. 2.13 ms by inputs and
+// clocks (under this load 1.9 GHz), 518 .. 566 TFLOP/s; 8 x 1056 tokens x 16 heads, no bias: 63 us, 580 TFLOP/s (79 with the training form's second term).
 // TRAIN: log-sum-exps, probabilities in two terms (with a table three), o_lo
 template <int BIAS, bool CAP, bool TRAIN>
 __global__ __launch_bounds__(256, 3) void pa_fwd_kernel(PAArgs p) {
@@ -521,8 +522,8 @@ __device__ __forceinline__ int dist_row(int d, int at) { return at / 128 + min(d
 
 constexpr int distn(int reach) { return 2 * reach + 1 + 2 * PADL; }
 
-// Lane layout and ring of the forward; dP beside the scores, dQ^T = K^T dS^T from the same K tile.  8 x 1056 tokens x 16 heads, no bias: 74 us; with a
-// table's gradient 117 us at 8397 tokens of 11 documents.
+// Lane layout and ring of the forward; dP beside the scores, dQ^T = K^T dS^T from the same K tile.  8 x 1056 tokens x 16 heads, no bias: 77 us; with a
+// table's gradient 113 us at 8397 tokens of 11 documents.
 // RG: 0 no table gradient, else the largest reach of this instantiation (its LDS)
 template <int BIAS, bool CAP, int RG>
 __global__ __launch_bounds__(256, (BIAS || CAP) ? 2 : 3) void pa_dq_kernel(PAArgs p) {
@@ -710,7 +711,7 @@ __global__ __launch_bounds__(256, (BIAS || CAP) ? 2 : 3) void pa_dq_kernel(PAArg
     }
 }
 
-// sums over the tiles of a head -> by_dist[h][2 R + 1]; 64 distances x 16 row groups per workgroup (6 us: latency of its dependent loads).  64 documents at a
+// sums over the tiles of a head -> by_dist[h][2 R + 1]; 64 distances x 16 row groups per workgroup (5 us: latency of its dependent loads).  64 documents at a
 // time: their rows are listed (a thread each finds its document by bisection), then added in the list's order
 __global__ __launch_bounds__(1024) void pa_dist_reduce_kernel(PAArgs p, float* by_dist) {
     __shared__ float sm[16][64];
@@ -777,8 +778,8 @@ __global__ __launch_bounds__(256) void pa_table_grad_kernel(const float* by_dist
 // One workgroup = 128 keys of one (document, key head); sweep over the 64-query tiles of all its query heads.  The query rows of the Q / dO tiles
 // are K-type images, so the accumulators (rows = queries) are the B operands of dV^T = dO^T P and dK^T = Q^T dS; their A operands come out of the
 // same tiles by transposing reads.  The 64 lse / delta values of a query tile ride along in the ring stage.  Two workgroups a CU (64 accumulators and
-// 32 operand registers a lane); 8 x 1056 tokens x 16 heads, no bias: 108 us, of which score products 18, output products 24, transposing reads 9, tile
-// copies 5, exp2 3 when each is left out alone: no single resource binds it.
+// 32 operand registers a lane); 8 x 1056 tokens x 16 heads, no bias: 111 us (matrix pipe and vector ALU 36 % each of the clocks in which a CU has work); of
+// 108 on one box score products 18, output products 24, transposing reads 9, tile copies 5, exp2 3 when each is left out alone: no single resource binds it.
 // Few key heads and tokens leave the chip's 512 slots for these workgroups empty: the sweep is then cut into `splits` parts whose fp32 sums a second
 // kernel adds in order (7392 tokens, 4 key heads of 16: 271 us whole, see splits_for for the rule).
 constexpr int KSTAGE = STAGE + 512;
