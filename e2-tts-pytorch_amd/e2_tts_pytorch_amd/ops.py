@@ -1113,12 +1113,12 @@ def _apart(out, q, k, v, what, in_place):
     mem = out.untyped_storage()
     lo = mem.data_ptr()
     hi = lo + mem.nbytes()
-    for t in (q, k, v):
+    for i, t in enumerate((q, k, v)):
         mem = t.untyped_storage()
         at = mem.data_ptr()
         if at >= hi or at + mem.nbytes() <= lo:               # (allocations of their own: the usual case, 3 us for all of it)
             continue
-        if t is q and in_place and out.data_ptr() == q.data_ptr() and all(n == 1 or x == y for n, x, y in zip(q.shape, q.stride(), out.stride())):
+        if i == 0 and in_place and out.data_ptr() == q.data_ptr() and all(n == 1 or x == y for n, x, y in zip(q.shape, q.stride(), out.stride())):
             continue
         if _rows_meet(out, t):
             raise E2KError(f'{what}: out shares memory with ' + ('k or v, or with q without being it' if in_place else 'q, k or v'))

@@ -73,6 +73,7 @@ def test_overlapping_outputs_are_refused(emu):
            lambda: f(q, k, v, cu, out=q, train=True), lambda: f(wide[:, :2], k, v, cu, out=wide[:, 1:3]), lambda: f(q, wide[:, :2], v, cu, out=wide[:, 1:3]),
            lambda: f(two[0].reshape(2, 16, 64).transpose(0, 1), k, v, cu, out=two[0]), lambda: f(q, k, v, cu, out=z(40, 64).as_strided((16, 2, 64), (128, 128, 1))),
            lambda: f(q, k, v, cu, out=z(40, 64).as_strided((16, 2, 64), (128, 64, 1), 64).as_strided((16, 2, 64), (128, 192, 1)))]
+    bad += [lambda: f(q, q, v, cu, out=q), lambda: f(q, k, q, cu, out=q), lambda: f(q, q, q, cu, out=q)]             # (q is k or v too)
     kc, L = z(3, 8, 2, 64), torch.ones(3, dtype=torch.int32)
     d, qs = ops.attn_decode, z(4, 2, 64)
     bad += [lambda: d(qs[:3], kc, kc.clone(), L, out=kc[:, 3]), lambda: d(qs[:3], kc.clone(), kc, L, out=kc[:, 7]), lambda: d(qs[:3], kc, kc, L, out=qs[1:]),
